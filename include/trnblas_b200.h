@@ -249,6 +249,72 @@ TRNBLAS_API int trnblas_pair_energy(int64_t nocc, int64_t nvir, int64_t naux, co
                         size_t workspace_bytes, void* stream);
 
 /*
+ * Products grouped by expert (no counterpart in the reference, whose batched
+ * products have entries of one size; they stand beside trnblas_gemm's batch).
+ * The first group_sizes[0] of the `rows` rows of A belong to group 0, the next
+ * group_sizes[1] to group 1 and so on: D[r] = alpha * A[r] @ op(B[g]) + beta *
+ * C[r] for a row r of group g, and D[r] = beta * C[r] (zero without C) for the
+ * rows behind the last group. A is rows x K, B a stack of `groups` matrices
+ * (K x N each, N x K when transB) strideB elements apart (0: one matrix for
+ * all), C and D rows x N of
+ * out_dtype, which is `dtype` (BF16 or F16; fp32 accumulate) or F32. The sizes
+ * are device int32 (sizes_64 = 0) or int64 and are read by the kernel: no host
+ * synchronisation, any of them may be zero. Negative sizes count as zero and
+ * sizes beyond `rows` are cut off; both leave code 8 in the status word. At
+ * most 1024 groups. The gradient of A is the same call on D's gradient with
+ * transB flipped. No workspace; D must not overlap A, B or C.
+ */
+TRNBLAS_API int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N,
+                         int64_t K, float alpha, const void* A, int64_t lda, const void* B,
+                         int64_t ldb, int64_t strideB, int transB, const void* group_sizes,
+                         int sizes_64, float beta, const void* C, int64_t ldc, void* D, int64_t ldd,
+                         void* stream);
+
+/*
+ * The gradient of trnblas_grouped_gemm's weights: D[g] = alpha * A_g^T @ B_g +
+ * beta * C[g], A_g (B_g) the rows of group g of the rows x M (rows x N)
+ * operand; beta * C[g] for a group without rows. C and D are stacks of
+ * `groups` M x N matrices of out_dtype. Nothing behind the last group is read
+ * into a result, infinities and NaN included.
+ */
+TRNBLAS_API int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t M,
+                               int64_t N, float alpha, const void* A, int64_t lda, const void* B,
+                               int64_t ldb, const void* group_sizes, int sizes_64, float beta,
+                               const void* C, int64_t ldc, int64_t strideC, void* D, int64_t ldd,
+                               int64_t strideD, void* stream);
+
+/*
+ * Microscaled 4-bit floating point (OCP MX, MXFP4): blocks of 32 values along
+ * K, each value E2M1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), each
+ * block with a power of two 2^(s - 127), s one byte. `data` holds two values a
+ * byte, the even one in the low half, rows ldq bytes apart (a multiple of 16,
+ * at least round_up(K, 32) / 2; K is padded with zeros); `scales` holds one
+ * 4-byte word for every row and 128 values of K, at [k / 128][row].
+ * s is the biased exponent of the block's largest magnitude less 2 (at least
+ * 0); values round to nearest, ties to the even mantissa, and saturate at 6.
+ * A block with an infinity or a NaN becomes s = 255: all NaN. X is F32, BF16
+ * or F16, rows x K, row stride ldx. trnblas_mxfp4_dequantize gives the values
+ * back in F32, BF16 or F16. No counterpart in the reference.
+ */
+TRNBLAS_API int trnblas_mxfp4_quantize(int dtype, int64_t rows, int64_t K, const void* X, int64_t ldx,
+                           void* data, int64_t ldq, void* scales, void* stream);
+TRNBLAS_API int trnblas_mxfp4_dequantize(int dtype, int64_t rows, int64_t K, const void* data, int64_t ldq,
+                             const void* scales, void* Y, int64_t ldy, void* stream);
+
+/*
+ * D[r] = alpha * A[r] @ B[g]^T + beta * C[r] on block-scaled 4-bit tensor
+ * cores, fp32 accumulate: A (rows x K) and B (`groups` stacked N x K matrices,
+ * quantised as one operand of groups * N rows) as trnblas_mxfp4_quantize
+ * writes them (lda, ldb in bytes), C and D rows x N of out_dtype (F32, BF16 or
+ * F16). group_sizes as for trnblas_grouped_gemm; NULL with groups = 1 is the
+ * dense product. No counterpart in the reference.
+ */
+TRNBLAS_API int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K,
+                       float alpha, const void* A, int64_t lda, const void* scalesA, const void* B,
+                       int64_t ldb, const void* scalesB, const void* group_sizes, int sizes_64,
+                       float beta, const void* C, int64_t ldc, void* D, int64_t ldd, void* stream);
+
+/*
  * Self-test of the bounded-wait machinery: launches one CTA that waits on an
  * mbarrier nothing will complete, with a `timeout_ns` bound, and returns.
  * The status word then holds the test's timeout code (6). No fault, no hang.

@@ -1,0 +1,147 @@
+"""Refusals of the grouped and 4-bit products, before any device work, and the
+host side of the packed format (CPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import trnblas_b200 as tb
+from oracle import experts as X
+from trnblas_b200 import _native as N
+
+BF = torch.bfloat16
+A, B, S = torch.zeros(6, 8, dtype=BF), torch.zeros(2, 8, 4, dtype=BF), torch.tensor([3, 3])
+
+
+def _mx(*shape):
+    *lead, K = shape
+    rows = 1
+    for n in lead:
+        rows *= n
+    return tb.MXFP4Tensor(torch.zeros(*lead, -(-K // 32) * 16, dtype=torch.uint8),
+                          torch.zeros(-(-K // 128), rows, 4, dtype=torch.uint8), shape)
+
+
+@pytest.mark.parametrize("call,exc", [
+    (lambda: tb.grouped_gemm(1.0, A.float(), B.float(), S), TypeError),
+    (lambda: tb.grouped_gemm(1.0, A, B.half(), S), RuntimeError),
+    (lambda: tb.grouped_gemm(1.0, A, B, S, out_dtype=torch.float16), TypeError),
+    (lambda: tb.grouped_gemm(1.0, A[0], B, S), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B[0], S), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, S, transB=True), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, S, transB="C"), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, [3, 3]), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, S.float()), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, S.view(1, 2)), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, torch.tensor([3, 2, 1])), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, torch.tensor([3, 4])), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B, torch.tensor([-1, 4])), ValueError),
+    (lambda: tb.grouped_gemm(1.0, A, B[:1].expand(1025, 8, 4), torch.zeros(1025, dtype=torch.int32)), ValueError),
+    (lambda: tb.grouped_gemm_wgrad(1.0, A, A[:5], S), ValueError),
+    (lambda: tb.grouped_gemm_wgrad(1.0, A, A.half(), S), RuntimeError),
+    (lambda: tb.grouped_gemm_wgrad(1.0, A, A, torch.tensor([3, 4])), ValueError),
+    (lambda: tb.grouped_gemm_wgrad(1.0, A, A, torch.zeros(1025, dtype=torch.int64)), ValueError),
+    (lambda: tb.quantize_mxfp4(A.double()), TypeError),
+    (lambda: tb.quantize_mxfp4(A[0]), ValueError),
+    (lambda: tb.dequantize_mxfp4(A), TypeError),
+    (lambda: tb.dequantize_mxfp4(_mx(3, 64), torch.float64), TypeError),
+    (lambda: tb.gemm_mxfp4(1.0, A, A), TypeError),
+    (lambda: tb.gemm_mxfp4(1.0, A.double(), _mx(3, 8)), TypeError),
+    (lambda: tb.gemm_mxfp4(1.0, A, _mx(3, 9)), ValueError),
+    (lambda: tb.gemm_mxfp4(1.0, A, _mx(2, 3, 8)), ValueError),
+    (lambda: tb.gemm_mxfp4(1.0, A, _mx(3, 8), out_dtype=torch.float64), TypeError),
+    (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(3, 8), S), ValueError),
+    (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), torch.tensor([6, 1])), ValueError),
+    (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), torch.tensor([6])), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(1, 3, 4, dtype=torch.uint8), (3, 33)), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16), torch.zeros(1, 3, 4, dtype=torch.uint8), (3, 32)), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(2, 3, 4, dtype=torch.uint8), (3, 32)), ValueError),
+    (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 16), torch.zeros(3, 1, dtype=torch.uint8), 32), TypeError),
+    (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 15, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 32), ValueError),
+    (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 2, dtype=torch.uint8), 32), ValueError),
+])
+def test_refused_before_device_work(call, exc):
+    with pytest.raises(exc):
+        call()
+
+
+FAKE = 1 << 20  # a non-NULL address that the argument checks reject before any use
+
+
+def test_c_entry_points_check_their_arguments():
+    L = N.lib()
+    ok = dict(dt=N.BF16, od=N.BF16, rows=4, G=2, n=8, k=8, a=FAKE, lda=8, b=FAKE, ldb=8, sb=64, tb=0, s=FAKE, c=None,
+              ldc=0, d=FAKE, ldd=8)
+
+    def grouped(**kw):
+        v = {**ok, **kw}
+        return L.trnblas_grouped_gemm(v["dt"], v["od"], v["rows"], v["G"], v["n"], v["k"], 1.0, v["a"], v["lda"], v["b"],
+                                      v["ldb"], v["sb"], v["tb"], v["s"], 0, 1.0, v["c"], v["ldc"], v["d"], v["ldd"], None)
+
+    for bad in (dict(dt=N.F32), dict(od=N.F16), dict(rows=-1), dict(G=1025), dict(s=None), dict(d=None), dict(ldd=7),
+                dict(a=None), dict(lda=7), dict(ldb=7), dict(sb=-8), dict(c=FAKE, ldc=7), dict(rows=1 << 31), dict(tb=1, k=16)):
+        assert grouped(**bad) == N.ERR_ARG, bad
+    assert grouped(rows=0) == 0 and grouped(n=0) == 0
+
+    def wgrad(**kw):
+        v = {**ok, **kw}
+        return L.trnblas_grouped_gemm_wgrad(v["dt"], v["od"], v["rows"], v["G"], v["k"], v["n"], 1.0, v["a"], v["lda"],
+                                            v["b"], v["ldb"], v["s"], 0, 1.0, v["c"], v["ldc"], 64, v["d"], v["ldd"],
+                                            v["sb"], None)
+
+    for bad in (dict(dt=N.F64), dict(od=N.F16), dict(G=-1), dict(s=None), dict(d=None), dict(ldd=7), dict(a=None),
+                dict(lda=7), dict(ldb=7), dict(sb=63), dict(c=FAKE, ldc=7)):
+        assert wgrad(**bad) == N.ERR_ARG, bad
+    assert wgrad(G=0) == 0
+
+    q = L.trnblas_mxfp4_quantize
+    for args in ((N.F64, 4, 8, FAKE, 8, FAKE, 16, FAKE), (N.F32, -1, 8, FAKE, 8, FAKE, 16, FAKE),
+                 (N.F32, 4, 8, FAKE, 7, FAKE, 16, FAKE), (N.F32, 4, 8, FAKE, 8, FAKE, 8, FAKE),
+                 (N.F32, 4, 33, FAKE, 33, FAKE, 16, FAKE), (N.F32, 4, 8, None, 8, FAKE, 16, FAKE),
+                 (N.F32, 4, 8, FAKE, 8, FAKE + 8, 16, FAKE), (N.F32, 4, 8, FAKE, 8, FAKE, 16, FAKE + 2)):
+        assert q(*args, None) == N.ERR_ARG, args
+    dq = L.trnblas_mxfp4_dequantize
+    for args in ((N.F64, 4, 8, FAKE, 16, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, FAKE, FAKE, 7),
+                 (N.F32, 4, 8, FAKE, 15, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, None, FAKE, 8)):
+        assert dq(*args, None) == N.ERR_ARG, args
+
+    def mx(od=N.BF16, rows=4, G=1, n=8, k=64, a=FAKE, lda=32, sa=FAKE, b=FAKE, ldb=32, sb=FAKE, s=None, c=None, ldc=0,
+           d=FAKE, ldd=8):
+        return L.trnblas_mxfp4_gemm(od, rows, G, n, k, 1.0, a, lda, sa, b, ldb, sb, s, 0, 1.0, c, ldc, d, ldd, None)
+
+    for bad in (dict(od=N.F64), dict(rows=-1), dict(G=2), dict(G=1025, s=FAKE), dict(d=None), dict(ldd=7), dict(lda=16),
+                dict(ldb=31), dict(a=None), dict(sa=FAKE + 1), dict(sb=None), dict(c=FAKE, ldc=7)):
+        assert mx(**bad) == N.ERR_ARG, bad
+    assert mx(rows=0) == 0
+
+
+@pytest.mark.parametrize("K", [1, 2, 31, 32, 33, 64, 127, 128, 129, 300])
+def test_parts_round_trip(K):
+    g = torch.Generator().manual_seed(K)
+    nb = -(-K // 32)
+    codes = torch.randint(0, 256, (2, 5, -(-K // 2)), dtype=torch.uint8, generator=g)
+    scales = torch.randint(0, 256, (2, 5, nb), dtype=torch.uint8, generator=g)
+    q = tb.MXFP4Tensor.from_parts(codes, scales, K)
+    assert q.shape == (2, 5, K) and q.dim() == 3
+    c, s = q.parts()
+    assert torch.equal(s, scales)
+    want = codes.clone()
+    if K % 2:
+        want[..., -1] &= 0x0F
+    assert torch.equal(c[..., : want.shape[-1]], want) and (c[..., want.shape[-1]:] == 0).all()
+    # word [k / 128][row] holds the row's four blocks there
+    words = q.scales
+    for r in range(10):
+        for b in range(4 * words.shape[0]):
+            v = words[b // 4, r, b % 4]
+            assert v == (scales.view(10, nb)[r, b] if b < nb else 0)
+
+
+def test_oracle_quantiser_by_hand():
+    x = torch.zeros(1, 64)
+    x[0, :9] = torch.tensor([4.0, 0.25, -0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9])
+    x[0, 32:35] = torch.tensor([2.0 ** -140, -(2.0 ** -128), 0.0])
+    v = X.dequantize(*X.quantize(x), 64)
+    assert v[0, :9].tolist() == [4.0, 0.0, -1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0]
+    assert v[0, 32:35].tolist() == [0.0, -(2.0 ** -128), 0.0]

@@ -1,0 +1,364 @@
+"""Products grouped by expert on a B200 against a plain 64-bit form: lengths
+from no row to many tiles, odd sizes, both layouts of the weights, the rows
+behind the last group, gradients, streams and captured graphs. The tolerance
+is derived in oracle/experts.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import trnblas_b200 as tb
+from oracle import experts as X
+
+pytestmark = pytest.mark.gpu
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda"
+
+
+def _rand(*shape, dt=BF, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed + 17 * len(shape) + sum(shape))
+    return torch.randn(*shape, device=DEV, generator=g).to(dt)
+
+
+def _sizes(s, dt=torch.int32):
+    return torch.tensor(s, dtype=dt, device=DEV)
+
+
+SIZES = [
+    [0],
+    [1],
+    [0, 0, 5, 0],
+    [300, 0, 1, 17],
+    [64, 65, 63, 1, 0, 128],
+    [513, 64, 0, 255, 256, 257],
+    [2] * 37,
+]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
+@pytest.mark.parametrize("transB", [False, True])
+@pytest.mark.parametrize("K,Nn", [(64, 128), (200, 264), (1032, 72), (65, 129), (1, 8), (8, 1), (7, 3)])
+def test_grouped_gemm(sizes, transB, K, Nn):
+    dt = BF if K % 2 == 0 else FP
+    rows = sum(sizes) + (K % 3) * 29
+    if rows == 0:
+        rows = 3
+    A = _rand(rows, K, dt=dt)
+    B = _rand(len(sizes), *((Nn, K) if transB else (K, Nn)), dt=dt)
+    for out in (dt, F32):
+        D = tb.grouped_gemm(1.0, A, B, _sizes(sizes), transB=transB, out_dtype=out)
+        ref, mags = X.grouped_gemm(1.0, A, B, sizes, transB=transB)
+        assert D.dtype == out and D.shape == ref.shape
+        X.check(D, ref, X.tolerance(ref, mags, K, out), f"{sizes} {K} {Nn} {out}")
+    assert tb.device_status(0) == 0
+
+
+def test_whole_numbers_are_exact():
+    """Small whole numbers: every partial sum is a whole number below 2^24, so
+    any association gives the same result, whatever the tiling."""
+    sizes = [700, 3, 0, 129, 31]
+    g = torch.Generator(device=DEV).manual_seed(5)
+    A = torch.randint(-8, 9, (sum(sizes), 520), device=DEV, generator=g).to(BF)
+    B = torch.randint(-8, 9, (5, 520, 328), device=DEV, generator=g).to(BF)
+    ref, _ = X.grouped_gemm(1.0, A, B, sizes)
+    assert torch.equal(tb.grouped_gemm(1.0, A, B, _sizes(sizes), out_dtype=F32).double(), ref)
+    dD = torch.randint(-8, 9, (sum(sizes), 328), device=DEV, generator=g).to(BF)
+    wref, _ = X.wgrad(1.0, A, dD, sizes)
+    assert torch.equal(tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes), out_dtype=F32).double(), wref)
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("out", ["same", "fp32"])
+@pytest.mark.parametrize("Nn", [256, 250])
+def test_alpha_beta_c(dt, out, Nn):
+    out = dt if out == "same" else F32
+    sizes, K = [40, 0, 333, 7], 136
+    rows = sum(sizes) + 21
+    A, B = _rand(rows, K, dt=dt), _rand(4, K, Nn, dt=dt)
+    C = _rand(rows, Nn, dt=out, seed=9)
+    ref, mags = X.grouped_gemm(-0.75, A, B, sizes, 0.5, C)
+    D = tb.grouped_gemm(-0.75, A, B, _sizes(sizes), 0.5, C)
+    if out != dt:
+        D = tb.grouped_gemm(-0.75, A, B, _sizes(sizes), 0.5, C, out_dtype=out)
+    tol = X.tolerance(ref, mags, K, out, C)
+    if D.dtype == out:
+        X.check(D, ref, tol)
+    # the rows behind the last group: beta * C, one rounding
+    X.check(D[-21:], 0.5 * C[-21:].double(), X.tolerance(ref, mags, 0, D.dtype, C)[-21:])
+    # beta = 0 reads no C
+    bad = torch.full_like(C, float("nan"))
+    assert torch.equal(tb.grouped_gemm(1.0, A, B, _sizes(sizes), 0.0, bad, out_dtype=out),
+                       tb.grouped_gemm(1.0, A, B, _sizes(sizes), out_dtype=out))
+    # strided C, and one that broadcasts (added after the product's rounding)
+    wide = _rand(rows, 2 * Nn, dt=out, seed=4)
+    r2, m2 = X.grouped_gemm(1.0, A, B, sizes, 2.0, wide[:, Nn:])
+    D2 = tb.grouped_gemm(1.0, A, B, _sizes(sizes), 2.0, wide[:, Nn:], out_dtype=out)
+    X.check(D2, r2, X.tolerance(r2, m2, K, out, 2.0 * wide[:, Nn:]))
+
+
+def test_strides_and_expanded_weights():
+    sizes, K, Nn = [9, 130, 0, 61], 96, 160
+    rows = sum(sizes)
+    big = _rand(rows, 3 * K)
+    A = big[:, K:2 * K]  # row stride 3K
+    At = _rand(K, rows).mT  # columns contiguous
+    one = _rand(1, K, Nn)
+    B = one.expand(4, K, Nn)
+    for a in (A, At, big[:, 1:K + 1]):  # the last one off 16 bytes
+        ref, mags = X.grouped_gemm(1.0, a, B, sizes)
+        X.check(tb.grouped_gemm(1.0, a, B, _sizes(sizes)), ref, X.tolerance(ref, mags, K, BF))
+    Bs = _rand(8, K, Nn)[::2]  # matrices two apart
+    ref, mags = X.grouped_gemm(1.0, A, Bs, sizes)
+    X.check(tb.grouped_gemm(1.0, A, Bs, _sizes(sizes)), ref, X.tolerance(ref, mags, K, BF))
+    w = tb.grouped_gemm_wgrad(1.0, At, big[:, 3:3 + K], _sizes(sizes))
+    ref, mags = X.wgrad(1.0, At, big[:, 3:3 + K], sizes)
+    X.check(w, ref, X.tolerance(ref, mags, max(sizes), BF))
+
+
+def test_sizes_on_host_64_bit_and_strided():
+    sizes = [5, 0, 90]
+    A, B = _rand(95, 64), _rand(3, 64, 64)
+    want = tb.grouped_gemm(1.0, A, B, _sizes(sizes))
+    assert torch.equal(want, tb.grouped_gemm(1.0, A, B, _sizes(sizes, torch.int64)))
+    assert torch.equal(want, tb.grouped_gemm(1.0, A, B, torch.tensor(sizes)))
+    pairs = torch.tensor([[5, 1], [0, 2], [90, 3]], device=DEV)
+    assert torch.equal(want, tb.grouped_gemm(1.0, A, B, pairs[:, 0]))
+    host = tb.grouped_gemm(1.0, A.cpu(), B.cpu(), torch.tensor(sizes))
+    assert host.device.type == "cpu" and torch.equal(host, want.cpu())
+
+
+def test_sizes_out_of_range_are_cut_off_and_reported():
+    A, B = _rand(100, 64), _rand(3, 64, 136)
+    assert tb.device_status(0) == 0
+    D = tb.grouped_gemm(1.0, A, B, _sizes([40, -7, 1 << 30]))
+    assert tb.device_status(0) == 8 and tb.device_status(0) == 0
+    assert torch.equal(D, tb.grouped_gemm(1.0, A, B, _sizes([40, 0, 60])))
+    W = tb.grouped_gemm_wgrad(1.0, A, A, _sizes([1 << 62, -(1 << 62), 1 << 62], torch.int64))
+    assert tb.device_status(0) == 8
+    assert torch.equal(W, tb.grouped_gemm_wgrad(1.0, A, A, _sizes([100, 0, 0])))
+    assert tb.device_status(0) == 0
+
+
+def test_nan_and_infinity_stay_in_their_rows_and_groups():
+    sizes, K, Nn = [50, 0, 83, 20], 192, 200
+    rows = sum(sizes) + 40
+    A, B = _rand(rows, K), _rand(4, K, Nn)
+    clean = tb.grouped_gemm(1.0, A, B, _sizes(sizes))
+    A2, B2 = A.clone(), B.clone()
+    A2[-40:] = float("nan")      # behind the last group
+    A2[60] = float("inf")        # one row of group 2
+    B2[1] = float("nan")         # a group without rows
+    B2[3] = float("inf")         # group 3
+    D = tb.grouped_gemm(1.0, A2, B2, _sizes(sizes))
+    keep = torch.ones(rows, dtype=torch.bool, device=DEV)
+    keep[60] = False
+    keep[133:153] = False
+    assert torch.equal(D[keep], clean[keep])
+    assert not D[60].isfinite().any() and not D[133:153].isfinite().any()
+    assert (D[-40:] == 0).all()
+    # the gradient of the weights: neighbours' rows are not even multiplied by zero
+    dD = _rand(rows, Nn, seed=3)
+    w = tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes))
+    A3, d3 = A.clone(), dD.clone()
+    A3[50:133], d3[50:133] = float("inf"), float("nan")  # group 2
+    A3[-40:], d3[-40:] = float("nan"), float("inf")
+    w3 = tb.grouped_gemm_wgrad(1.0, A3, d3, _sizes(sizes))
+    for g in (0, 1, 3):
+        assert torch.equal(w3[g], w[g]), g
+    assert w3[2].isnan().all() and (w3[1] == 0).all()
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
+@pytest.mark.parametrize("M,Nn", [(64, 128), (200, 264), (136, 1000), (65, 129), (1, 1)])
+def test_wgrad(sizes, M, Nn):
+    dt = FP if M % 2 else BF
+    rows = sum(sizes) + (M % 3) * 13
+    A, B = _rand(rows, M, dt=dt), _rand(rows, Nn, dt=dt, seed=2)
+    for out in (dt, F32):
+        D = tb.grouped_gemm_wgrad(0.5, A, B, _sizes(sizes), out_dtype=out)
+        ref, mags = X.wgrad(0.5, A, B, sizes)
+        assert D.dtype == out and D.shape == ref.shape
+        X.check(D, ref, X.tolerance(ref, mags, max(sizes), out), f"{sizes} {M} {Nn} {out}")
+    C = _rand(len(sizes), M, Nn, dt=F32, seed=7)
+    ref, mags = X.wgrad(1.0, A, B, sizes, 1.0, C)
+    D = tb.grouped_gemm_wgrad(1.0, A, B, _sizes(sizes), 1.0, C, out_dtype=F32)
+    X.check(D, ref, X.tolerance(ref, mags, max(sizes), F32, C))
+    for g, m in enumerate(sizes):
+        if m == 0:
+            assert torch.equal(D[g], C[g])
+
+
+def test_no_rows_no_groups():
+    B = _rand(3, 64, 32)
+    assert tb.grouped_gemm(1.0, _rand(0, 64), B, _sizes([0, 0, 0])).shape == (0, 32)
+    assert (tb.grouped_gemm(1.0, _rand(7, 64), _rand(0, 64, 32), _sizes([])) == 0).all()
+    C = _rand(7, 32)
+    assert torch.equal(tb.grouped_gemm(1.0, _rand(7, 0), _rand(3, 0, 32), _sizes([7, 0, 0]), 1.0, C), C)
+    C3 = _rand(3, 8, 16)
+    assert torch.equal(tb.grouped_gemm_wgrad(1.0, _rand(0, 8), _rand(0, 16), _sizes([0, 0, 0]), 1.0, C3), C3)
+    assert tb.grouped_gemm_wgrad(1.0, _rand(5, 8), _rand(5, 16), _sizes([])).shape == (0, 8, 16)
+
+
+@pytest.mark.parametrize("transB", [False, True])
+@pytest.mark.parametrize("shared", [False, True])
+def test_gradients_against_the_formula(transB, shared):
+    sizes, K, Nn = [70, 0, 130, 9], 128, 96
+    rows = sum(sizes) + 5
+    shape = (Nn, K) if transB else (K, Nn)
+    A = _rand(rows, K).requires_grad_()
+    W = (_rand(1, *shape) if shared else _rand(4, *shape)).requires_grad_()
+    B = W.expand(4, *shape)
+    C = _rand(rows, Nn, seed=5).requires_grad_()
+    dD = _rand(rows, Nn, seed=6)
+    D = tb.grouped_gemm(0.5, A, B, _sizes(sizes), 2.0, C, transB=transB)
+    assert torch.equal(D.detach(), tb.grouped_gemm(0.5, A.detach(), B.detach(), _sizes(sizes), 2.0, C.detach(),
+                                                  transB=transB))
+    dA, dW, dC = torch.autograd.grad(D, (A, W, C), dD)
+    ra, ma = X.grouped_gemm(0.5, dD, B.detach(), sizes, transB=not transB)
+    X.check(dA, ra, X.tolerance(ra, ma, Nn, BF))
+    l, r = (dD, A.detach()) if transB else (A.detach(), dD)
+    rw, mw = X.wgrad(0.5, l, r, sizes)
+    assert dW.shape == W.shape
+    if shared:  # the groups' gradients, each rounded to bf16, summed by torch in bf16 with fp32 sums
+        tol = X.tolerance(rw, mw, max(sizes), BF).sum(0, keepdim=True)
+        rw = rw.sum(0, keepdim=True)
+        X.check(dW, rw, tol + 2.0 ** -8 * (rw.abs() + tol))
+    else:
+        X.check(dW, rw, X.tolerance(rw, mw, max(sizes), BF))
+    assert torch.equal(dC, 2.0 * dD)
+
+
+def test_gradients_against_differences():
+    """The product is linear in each operand: with whole numbers the
+    difference over a unit step is exact in fp32 and is the gradient."""
+    sizes, K, Nn = [33, 0, 20], 40, 24
+    rows = sum(sizes) + 4
+    g = torch.Generator(device=DEV).manual_seed(1)
+    A = torch.randint(-4, 5, (rows, K), device=DEV, generator=g).to(BF).requires_grad_()
+    B = torch.randint(-4, 5, (3, K, Nn), device=DEV, generator=g).to(BF).requires_grad_()
+    w = torch.randint(-3, 4, (rows, Nn), device=DEV, generator=g).to(F32)
+    s = _sizes(sizes)
+
+    def loss(a, b):
+        return (tb.grouped_gemm(1.0, a, b, s, out_dtype=F32).double() * w).sum()
+
+    dA, dB = torch.autograd.grad(loss(A, B), (A, B))
+    base = loss(A.detach(), B.detach())
+    for r, k in [(0, 0), (32, 39), (33, 5), (52, 17), (53, 3), (56, 39)]:
+        a = A.detach().clone()
+        a[r, k] += 1
+        assert loss(a, B.detach()) - base == dA[r, k].double(), (r, k)
+    for e, k, n in [(0, 0, 0), (0, 39, 23), (1, 4, 4), (2, 7, 11)]:
+        b = B.detach().clone()
+        b[e, k, n] += 1
+        assert loss(A.detach(), b) - base == dB[e, k, n].double(), (e, k, n)
+
+
+def test_layer_forward_and_backward():
+    """The operators as a layer uses them: tokens sorted by expert, two grouped
+    products with a gate between them, gradients through both. Every product is
+    checked against 64 bits on the very operands it got."""
+    tokens, dim, hidden, G = 301, 128, 192, 6
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(tokens, dim, device=DEV, generator=g).to(BF).requires_grad_()
+    w1 = (torch.randn(G, hidden, dim, device=DEV, generator=g) * dim ** -0.5).to(BF).requires_grad_()
+    w2 = (torch.randn(G, dim, hidden, device=DEV, generator=g) * hidden ** -0.5).to(BF).requires_grad_()
+    expert = torch.randint(0, G - 1, (tokens,), device=DEV, generator=g)  # the last one gets none
+    order = torch.argsort(expert, stable=True)
+    sizes = torch.bincount(expert, minlength=G)
+    xs = x[order]
+    h = tb.grouped_gemm(1.0, xs, w1, sizes, transB=True)
+    a = torch.relu(h)
+    y = tb.grouped_gemm(1.0, a, w2, sizes, transB=True)
+    dy = torch.randn(tokens, dim, device=DEV, generator=g).to(BF)
+    gx, g1, g2, gh = torch.autograd.grad(y, (x, w1, w2, h), dy)
+    sz = sizes.tolist()
+    for out, ops, terms in (
+        (h, (xs.detach(), w1.detach(), True), dim),
+        (y, (a.detach(), w2.detach(), True), hidden),
+    ):
+        ref, mags = X.grouped_gemm(1.0, ops[0], ops[1], sz, transB=ops[2])
+        X.check(out.detach(), ref, X.tolerance(ref, mags, terms, BF))
+    ref, mags = X.wgrad(1.0, dy, a.detach(), sz)
+    X.check(g2, ref, X.tolerance(ref, mags, max(sz), BF))
+    ref, mags = X.grouped_gemm(1.0, dy, w2.detach(), sz)
+    ok = h.detach() > 0
+    X.check(torch.where(ok, gh, 0), torch.where(ok, ref, 0), X.tolerance(ref, mags, dim, BF))
+    ref, mags = X.wgrad(1.0, gh, xs.detach(), sz)
+    X.check(g1, ref, X.tolerance(ref, mags, max(sz), BF))
+    ref, mags = X.grouped_gemm(1.0, gh, w1.detach(), sz)
+    inv = torch.empty_like(order)
+    inv[order] = torch.arange(tokens, device=DEV)
+    X.check(gx, ref[inv], X.tolerance(ref, mags, hidden, BF)[inv])
+    assert (g1[G - 1] == 0).all() and (g2[G - 1] == 0).all()
+
+
+def test_captured_graph_follows_the_sizes():
+    sizes = _sizes([10, 50, 4, 0])
+    A, B = _rand(90, 128), _rand(4, 128, 136)
+    dD = _rand(90, 136, seed=1)
+    tb.grouped_gemm(1.0, A, B, sizes)
+    tb.grouped_gemm_wgrad(1.0, A, dD, sizes)
+    torch.cuda.synchronize()
+    graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        D = tb.grouped_gemm(1.0, A, B, sizes)
+        dA = tb.grouped_gemm(1.0, dD, B, sizes, transB=True)
+        W = tb.grouped_gemm_wgrad(1.0, A, dD, sizes)
+    with torch.cuda.graph(graph2):
+        D2 = tb.grouped_gemm(2.0, A, B, sizes)
+    for s in ([10, 50, 4, 0], [0, 0, 0, 90], [0, 0, 0, 0], [1, 88, 0, 1]):
+        sizes.copy_(torch.tensor(s, dtype=torch.int32))
+        A.copy_(_rand(90, 128, seed=s[1]))
+        graph.replay()
+        graph2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(D, tb.grouped_gemm(1.0, A, B, _sizes(s)))
+        assert torch.equal(D2, tb.grouped_gemm(2.0, A, B, _sizes(s)))
+        assert torch.equal(dA, tb.grouped_gemm(1.0, dD, B, _sizes(s), transB=True))
+        assert torch.equal(W, tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(s)))
+    assert tb.device_status(0) == 0
+
+
+def test_two_streams_and_the_same_result_twice():
+    sizes = [700, 0, 33, 290]
+    A, B, s = _rand(1023, 512), _rand(4, 512, 640), _sizes(sizes)
+    dD = _rand(1023, 640)
+    want, wantw = tb.grouped_gemm(1.0, A, B, s), tb.grouped_gemm_wgrad(1.0, A, dD, s)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append((tb.grouped_gemm(1.0, A, B, s), tb.grouped_gemm_wgrad(1.0, A, dD, s)))
+    torch.cuda.synchronize()
+    for d, w in outs:
+        assert torch.equal(d, want) and torch.equal(w, wantw)
+
+
+def test_offsets_past_32_bits():
+    """A result of 2.3 G elements: the last rows sit behind 2^31 elements."""
+    rows, K, Nn = 71000, 64, 32768
+    A, B = _rand(rows, K), _rand(2, K, Nn)
+    sizes = [70000, 900]
+    D = tb.grouped_gemm(1.0, A, B, _sizes(sizes))
+    for r0, r1, g in ((0, 40, 0), (69960, 70000, 0), (70000, 70040, 1), (70860, 70900, 1)):
+        ref, mags = X.grouped_gemm(1.0, A[r0:r1], B[g:g + 1], [r1 - r0])
+        X.check(D[r0:r1], ref, X.tolerance(ref, mags, K, BF))
+    assert (D[70900:] == 0).all()
+    del D
+    W = tb.grouped_gemm_wgrad(1.0, A[:256], _rand(256, 2 * Nn), _sizes([100, 156] + [0] * 1000 + [0]), out_dtype=BF)
+    assert (W[2:] == 0).all()
+
+
+def test_many_groups():
+    G = 1024
+    sizes = [(i * 7) % 5 for i in range(G)]
+    A, B = _rand(sum(sizes), 64), _rand(G, 64, 40)
+    ref, mags = X.grouped_gemm(1.0, A, B, sizes)
+    X.check(tb.grouped_gemm(1.0, A, B, _sizes(sizes)), ref, X.tolerance(ref, mags, 64, BF))
+    dD = _rand(sum(sizes), 40)
+    ref, mags = X.wgrad(1.0, A, dD, sizes)
+    X.check(tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes)), ref, X.tolerance(ref, mags, 5, BF))

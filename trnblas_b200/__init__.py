@@ -12,12 +12,16 @@ from . import _native
 from ._flags import diag_flag, side_flag, trans_flag, uplo_flag
 from . import energy, ops, parallel
 from .energy import batched_pair_energy, nki_batched_pair_energy, pair_range_energy
+from .experts import grouped_gemm, grouped_gemm_wgrad
 from .level3 import batched_gemm, gemm, gemm_fp64, metric_inv_half, symm, syrk, trmm, trsm
+from .mxfp4 import MXFP4Tensor, dequantize_mxfp4, gemm_mxfp4, grouped_gemm_mxfp4, quantize_mxfp4
 
 __version__ = "0.1.0"
 
 __all__ = [
     "gemm", "batched_gemm", "syrk", "gemm_fp64", "trsm", "metric_inv_half", "symm", "trmm",
+    "grouped_gemm", "grouped_gemm_wgrad", "MXFP4Tensor", "quantize_mxfp4", "dequantize_mxfp4",
+    "gemm_mxfp4", "grouped_gemm_mxfp4",
     "batched_pair_energy", "nki_batched_pair_energy", "pair_range_energy",
     "energy", "ops", "parallel",
     "trans_flag", "uplo_flag", "side_flag", "diag_flag",

@@ -72,6 +72,18 @@ _SIGNATURES = {
     "trnblas_pair_energy": (
         _i, [_i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _sz, _p]
     ),
+    "trnblas_grouped_gemm": (
+        _i, [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i64, _i, _p, _i, _f, _p, _i64, _p, _i64, _p]
+    ),
+    "trnblas_grouped_gemm_wgrad": (
+        _i,
+        [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p, _i, _f, _p, _i64, _i64, _p, _i64, _i64, _p],
+    ),
+    "trnblas_mxfp4_quantize": (_i, [_i, _i64, _i64, _p, _i64, _p, _i64, _p, _p]),
+    "trnblas_mxfp4_dequantize": (_i, [_i, _i64, _i64, _p, _i64, _p, _p, _i64, _p]),
+    "trnblas_mxfp4_gemm": (
+        _i, [_i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _p, _i64, _p, _p, _i, _f, _p, _i64, _p, _i64, _p]
+    ),
     "trnblas_wait_selftest": (_i, [ctypes.c_ulonglong, _p]),
 }
 

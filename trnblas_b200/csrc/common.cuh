@@ -41,6 +41,7 @@ enum Status : int {
   kTimeoutDrain = 5,    // exit path could not drain in-flight copies
   kTimeoutTest = 6,     // the deliberate short wait of the status self-test
   kTimeoutAux = 7,      // converter / auxiliary warp wait
+  kBadGroups = 8,       // group sizes negative or beyond the rows (cut off)
 };
 
 // Default bound for one wait: 4 s. A healthy wait lasts microseconds; the bound

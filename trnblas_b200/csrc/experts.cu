@@ -1,0 +1,145 @@
+// C-ABI entry points of the products grouped by expert, 16-bit: the forward
+// product (and with op(B) flipped the gradient of its rows) and the gradient
+// of the weights.
+#include <algorithm>
+
+#include "experts_host.hpp"
+#include "experts_wgrad_sm100.cuh"
+
+namespace tb {
+namespace {
+
+int check_grouped(const char* what, int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N,
+                  int64_t K, const void* sizes) {
+  const std::string w(what);
+  if (dtype != TRNBLAS_BF16 && dtype != TRNBLAS_F16) {
+    set_error(w + ": dtype must be BF16 or F16");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (out_dtype != dtype && out_dtype != TRNBLAS_F32) {
+    set_error(w + ": the output is of the operands' dtype or F32");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (int rc = check_group_dims(what, rows, groups, N, K)) return rc;
+  if (groups > 0 && rows > 0 && !sizes) {
+    set_error(w + ": NULL group sizes");
+    return TRNBLAS_ERR_ARG;
+  }
+  return TRNBLAS_OK;
+}
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" {
+
+int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K,
+                         float alpha, const void* A, int64_t lda, const void* B, int64_t ldb,
+                         int64_t strideB, int transB, const void* group_sizes, int sizes_64, float beta,
+                         const void* C, int64_t ldc, void* D, int64_t ldd, void* stream) {
+  if (int rc = check_grouped("trnblas_grouped_gemm", dtype, out_dtype, rows, groups, N, K, group_sizes))
+    return rc;
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  if (!D || ldd < N || (C && beta != 0.0f && ldc < N)) {
+    set_error("trnblas_grouped_gemm: NULL output, or ldc/ldd smaller than N");
+    return TRNBLAS_ERR_ARG;
+  }
+  // no products at all: D = beta * C
+  if (K == 0 || groups == 0)
+    return trnblas_gemm(out_dtype, 1, rows, N, 0, alpha, nullptr, 1, 0, 0, nullptr, N, 0, 0, beta, C, ldc, 0,
+                        D, ldd, 0, nullptr, 0, stream);
+  const int64_t b_rows = transB ? N : K, b_cols = transB ? K : N;
+  if (!A || !B || lda < K || ldb < b_cols || strideB < 0) {
+    set_error("trnblas_grouped_gemm: NULL operand, or a stride smaller than the row length");
+    return TRNBLAS_ERR_ARG;
+  }
+  const auto dt = dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const bool shared = groups == 1 || strideB == 0;  // one matrix
+  const int64_t nb = shared ? 1 : groups, sb = shared ? round_up(ldb * b_rows, 8) : strideB;
+  const int64_t sa = round_up(lda * rows, 8);
+  // Row tiles of 64 where a group has at most 48 rows on average: eight
+  // pipeline stages instead of four keep more weight bytes in flight, which is
+  // what bounds a few rows a group.
+  const bool small = rows <= 48 * groups;
+  CUtensorMap mw, mx, mx64;
+  const bool ok = (transB ? encode_map_3d(&mw, dt, 2, B, K, N, nb, ldb, sb, 64, 128)
+                          : encode_map_3d(&mw, dt, 2, B, N, K, nb, ldb, sb, 64, 64)) &&
+                  encode_map_3d(&mx, dt, 2, A, K, rows, 1, lda, sa, 64, small ? 64 : 256) &&
+                  encode_map_3d(&mx64, dt, 2, A, K, rows, 1, lda, sa, 64, 64);
+  if (!ok) return TRNBLAS_ERR_ALIGN;
+  ExpertsParams p{};
+  if (int rc = fill_experts(p, out_dtype, rows, groups, N, K, alpha, group_sizes, sizes_64, beta, C, ldc, D, ldd))
+    return rc;
+  p.in_fmt = dtype == TRNBLAS_BF16 ? kFmtBF16 : kFmtF16;
+  p.w_mn = transB ? 0 : 1;
+  p.w_shared = shared;
+  return small ? launch_experts<kExpF16, 64>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream))
+               : launch_experts<kExpF16, 256>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream));
+}
+
+int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t M, int64_t N,
+                               float alpha, const void* A, int64_t lda, const void* B, int64_t ldb,
+                               const void* group_sizes, int sizes_64, float beta, const void* C, int64_t ldc,
+                               int64_t strideC, void* D, int64_t ldd, int64_t strideD, void* stream_) {
+  if (int rc = check_grouped("trnblas_grouped_gemm_wgrad", dtype, out_dtype, rows, groups, N, M, group_sizes))
+    return rc;
+  if (groups == 0 || M == 0 || N == 0) return TRNBLAS_OK;
+  const bool has_c = C && beta != 0.0f;
+  if (!D || ldd < N || (has_c && ldc < N) ||
+      (groups > 1 && (strideD < ldd * M || (has_c && strideC < 0)))) {
+    set_error("trnblas_grouped_gemm_wgrad: NULL output, or a C / D stride smaller than what it steps over");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (rows == 0)
+    return trnblas_gemm(out_dtype, groups, M, N, 0, alpha, nullptr, 1, 0, 0, nullptr, N, 0, 0, beta, C, ldc,
+                        strideC, D, ldd, strideD, nullptr, 0, stream_);
+  if (!A || !B || lda < M || ldb < N) {
+    set_error("trnblas_grouped_gemm_wgrad: NULL operand, or lda/ldb smaller than the row length");
+    return TRNBLAS_ERR_ARG;
+  }
+  using Cfg = WgradCfg;
+  const auto dt = dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!encode_map_3d(&ma, dt, 2, A, M, rows, 1, lda, round_up(lda * rows, 8), 64, 64) ||
+      !encode_map_3d(&mb, dt, 2, B, N, rows, 1, ldb, round_up(ldb * rows, 8), 64, 64))
+    return TRNBLAS_ERR_ALIGN;
+  WgradParams w{};
+  w.p.tiles_m = static_cast<int>(ceil_div(M, Cfg::BM));
+  w.p.tiles_n = static_cast<int>(ceil_div(N, Cfg::BN));
+  const long long tiles = groups * static_cast<long long>(w.p.tiles_m) * w.p.tiles_n;
+  if (tiles > (1ll << 30)) {
+    set_error("trnblas_grouped_gemm_wgrad: too many tiles");
+    return TRNBLAS_ERR_ARG;
+  }
+  w.p.M = static_cast<int>(M);
+  w.p.N = static_cast<int>(N);
+  w.p.out_kind = out_kind_of(out_dtype);
+  w.p.c_mode = has_c ? kCRow : kCNone;
+  w.p.alpha = alpha;
+  w.p.beta = beta;
+  w.p.C = C;
+  w.p.ldc = ldc;
+  w.p.strideC = strideC;
+  w.p.D = D;
+  w.p.ldd = ldd;
+  w.p.strideD = strideD;
+  w.p.num_tiles = static_cast<int>(tiles);
+  w.p.status = status_word();
+  if (!w.p.status) return TRNBLAS_ERR_CUDA;
+  w.p.timeout_ns = wait_timeout_ns();
+  w.rows = static_cast<int>(rows);
+  w.groups = static_cast<int>(groups);
+  w.sizes = group_sizes;
+  w.sizes64 = sizes_64;
+  w.in_fmt = dtype == TRNBLAS_BF16 ? kFmtBF16 : kFmtF16;
+  static bool attr_set[64] = {};
+  if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_kernel), Cfg::SMEM, attr_set)) return rc;
+  const int grid = static_cast<int>(std::min<long long>(tiles, num_sms()));
+  wgrad_kernel<<<grid, Cfg::THREADS, Cfg::SMEM, static_cast<cudaStream_t>(stream_)>>>(ma, mb, w);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "weight gradient kernel launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,555 @@
+// Products grouped by expert, sm_100a: rows of A that belong to group g
+// multiply matrix g of a stack of weights, groups of any length.
+//
+//   forward  D[r] = alpha * A[r] op(W[g]) + beta * C[r]     (experts_kernel)
+//   wgrad    D[g] = alpha * A_g^T B_g + beta * C[g]         (experts_wgrad_sm100.cuh)
+//
+// The group sizes are read on the device: every CTA scans them once into a
+// table of first rows and first tiles in shared memory (G <= kMaxGroups), then
+// walks its tiles with a static stride. Sizes below zero count as zero and
+// rows past the operand's end are cut off (recorded in the status word), so no
+// index leaves the operands whatever the sizes hold.
+//
+// Forward: the weights are the M side of the MMA (128 of their output columns
+// on the 128 TMEM lanes) and the rows of A the N side. An MMA's time goes with
+// N, which may be any multiple of 16, so a group of m rows costs
+// round_up(m, 16) whatever the tile size: groups of one row and of thousands
+// run on the same kernel, and a group's rows are cut into equal tiles instead
+// of full ones and a remainder. The epilogue turns 32 x 32 blocks through
+// shared memory, since TMEM lanes run along a row of D.
+//
+// Operand kinds of the forward kernel:
+//   kExpF16  bf16 / fp16, fp32 accumulate; weights stored N x K (K-major) or
+//            K x N (MN-major), no transposed copy;
+//   kExpMx4  E2M1 pairs with one power of two per 32 values along K
+//            (kind::mxf4, block scaled by the tensor core): two scale warps
+//            bring the scale words by 4-byte cp.async straight into the
+//            32 x 16-byte order that tcgen05.cp copies to TMEM, so rows may
+//            start anywhere. Each pipeline stage has its own TMEM scale
+//            columns, which its empty barrier frees with the stage.
+#pragma once
+
+#include "gemm_sm100.cuh"
+
+namespace tb {
+
+enum ExpKind : int { kExpF16 = 0, kExpMx4 = 1 };
+constexpr int kMaxGroups = 1024;
+
+struct GroupTable {
+  int* row0;   // [G + 2] first row of each group; [G] the rows behind the last group, [G + 1] rows
+  int* tile0;  // [G + 2] first tile; [G + 1] all tiles
+};
+
+struct ExpertsParams {
+  int rows, N, K;
+  int groups;
+  const void* sizes;  // device, int32 or int64; nullptr: one group of all rows
+  int sizes64;
+  int in_fmt;   // kExpF16: kFmtBF16 / kFmtF16
+  int w_mn;     // kExpF16: weights stored K x N
+  int w_shared; // kExpF16: one matrix for every group
+  int out_kind;
+  float alpha, beta;
+  const void* C;
+  long long ldc;
+  void* D;
+  long long ldd;
+  int tiles_w;  // weight tiles of 128
+  // kExpMx4: scale words [K / 128][rows] of the rows and of the weights
+  const uint32_t* xs;
+  long long xs_rows;
+  const uint32_t* ws;
+  long long ws_rows;
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ long long load_size(const void* sizes, int sizes64, int g) {
+  return sizes64 ? __ldg(reinterpret_cast<const long long*>(sizes) + g)
+                 : static_cast<long long>(__ldg(reinterpret_cast<const int*>(sizes) + g));
+}
+
+// One warp: the first row of every group, and the first tile with `bn` rows to
+// a tile at most and `per` tiles for each of them (bn 0: rows only).
+__device__ __forceinline__ void build_groups(const GroupTable& tb, const void* sizes, int sizes64,
+                                             int groups, int rows, int bn, int per, int* status) {
+  const int lane = threadIdx.x & 31;
+  long long run = 0;
+  int tiles = 0;
+  bool bad = false;
+  for (int base = 0; base < groups; base += 32) {
+    const int g = base + lane;
+    long long s = 0;
+    if (g < groups) s = sizes ? load_size(sizes, sizes64, g) : rows;
+    bad |= s < 0;
+    s = s < 0 ? 0 : (s > rows ? static_cast<long long>(rows) + 1 : s);
+    long long inc = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const long long end = run + inc;
+    const int hi = static_cast<int>(end < rows ? end : rows);
+    const int lo = static_cast<int>(end - s < rows ? end - s : rows);
+    const int nt = bn ? ((hi - lo + bn - 1) / bn) * per : 0;
+    int tinc = nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, tinc, o);
+      if (lane >= o) tinc += u;
+    }
+    if (g < groups) {
+      tb.row0[g] = lo;
+      if (bn) tb.tile0[g] = tiles + tinc - nt;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+    tiles += __shfl_sync(0xffffffffu, tinc, 31);
+  }
+  bad |= run > rows;
+  if (__any_sync(0xffffffffu, bad) && blockIdx.x == 0 && lane == 0)
+    atomicCAS(status, 0, static_cast<int>(kBadGroups));
+  if (lane == 0) {
+    const int end = static_cast<int>(run < rows ? run : rows);
+    tb.row0[groups] = end;
+    tb.row0[groups + 1] = rows;
+    if (bn) {
+      tb.tile0[groups] = tiles;
+      tb.tile0[groups + 1] = tiles + ((rows - end + bn - 1) / bn) * per;
+    }
+  }
+}
+
+struct ExpTile {
+  int g;       // group, or `groups` for the rows behind the last one
+  int r0, nv;  // first row and number of rows
+  int n0;      // first weight column
+};
+
+// Tile t: the tiles of one weight block are next to one another, so the CTAs
+// that run together share it and the group's rows.
+template <int BN>
+__device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, int t) {
+  int lo = 0, hi = groups + 1;  // tile0[lo] <= t < tile0[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tb.tile0[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  ExpTile e;
+  e.g = lo;
+  const int first = tb.row0[lo], m = tb.row0[lo + 1] - first;
+  const int nt = (m + BN - 1) / BN;
+  // equal tiles, a multiple of 16 rows each (the last one keeps the rest;
+  // never empty, since nt - 1 tiles of at most BN rows do not cover m)
+  const int step = ((m + nt - 1) / nt + 15) & ~15;
+  const int i = t - tb.tile0[lo];
+  const int w = i / nt, x = i - w * nt;
+  e.r0 = first + x * step;
+  e.nv = min(step, m - x * step);
+  e.n0 = w * 128;
+  return e;
+}
+
+template <int KIND, int BN>
+struct ExpCfg {
+  static constexpr bool MX = KIND == kExpMx4;
+  static constexpr int BK = MX ? 256 : 64;  // one 128-byte swizzle row of K
+  static constexpr int W_TILE = 128 * 128;
+  static constexpr int X_TILE = BN * 128;
+  static constexpr int XBLK = (BN + 127) / 128;       // 128-row scale blocks of the rows
+  static constexpr int SFW = MX ? 2 * 512 : 0;        // two scale words (K = 128 each)
+  static constexpr int SFX = MX ? 2 * XBLK * 512 : 0;
+  static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
+  static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle atom's alignment");
+  // what fits beside 16 KB of epilogue blocks and the group table; at most 8
+  static constexpr int FIT = (227 * 1024 - 1024 - 512 - kEpiStageBytes - (kMaxGroups + 2) * 8) / STAGE_BYTES;
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int SF_COLS = MX ? 2 * 4 * (1 + XBLK) : 0;  // TMEM scale columns of a stage
+  static constexpr int COLS = 2 * BN + STAGES * SF_COLS;
+  static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static_assert(COLS <= 512, "accumulators and scales fit TMEM");
+  static constexpr int SCALE_WARPS = MX ? 2 : 0;
+  static constexpr int THREADS = 32 * (6 + SCALE_WARPS);
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + kEpiStageBytes + (kMaxGroups + 2) * 8;
+};
+
+// Instruction descriptor of kind::mxf4 with E8M0 scales: E2M1 operands, N / 8
+// at bit 17, the scale type at 23, M / 128 at 27, the scale bytes' position in
+// their words (0 or 2) at bits 4 and 29.
+__host__ __device__ constexpr uint32_t idesc_mx4(uint32_t N, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | (1u << 27) | (sf << 29);
+}
+
+__device__ __forceinline__ void mma_mx4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows x 16 bytes of shared memory into 4 TMEM columns, the same in all
+// four lane quarters: the scale words of 128 rows, word of row r at lane
+// r % 32, column r / 32.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
+// 4 bytes global -> shared, zero when !ok (src is not read then).
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
+  const uint32_t n = ok ? 4u : 0u;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Forward epilogue of one warp's block: lane l holds v[j] = accumulator of
+// weight column n0 + l (n0: the warp's first) and row r0 + j, j < left.
+__device__ __forceinline__ void exp_store(const ExpertsParams& p, int r0, int left, int n0,
+                                          const float* v, void* tsm) {
+  const int lane = threadIdx.x & 31;
+  const int n = n0 + lane;
+  const bool has_c = p.C != nullptr && p.beta != 0.0f;
+  float out[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) out[j] = p.alpha * v[j];
+  if (has_c && n < p.N) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) out[j] += p.beta * load_c(p.C, p.out_kind, (r0 + static_cast<long long>(j)) * p.ldc + n);
+  }
+  const bool wide = (reinterpret_cast<uintptr_t>(p.D) & 15) == 0 && n0 + 32 <= p.N;
+  if (p.out_kind == kOutF32) {
+    if (wide && p.ldd % 4 == 0) {
+      float* T = reinterpret_cast<float*>(tsm);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) T[j * 32 + lane] = out[j];
+      __syncwarp();
+      const int q4 = (lane & 7) * 4;
+      float* D = reinterpret_cast<float*>(p.D) + n0 + q4;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int row = 4 * k + (lane >> 3);
+        if (row < left)
+          *reinterpret_cast<float4*>(D + (r0 + static_cast<long long>(row)) * p.ldd) =
+              *reinterpret_cast<const float4*>(&T[row * 32 + q4]);
+      }
+      __syncwarp();  // the block is rewritten by the next chunk
+      return;
+    }
+  } else if (wide && p.ldd % 8 == 0) {
+    unsigned short* T = reinterpret_cast<unsigned short*>(tsm);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      T[j * 32 + lane] = (p.out_kind == kOutBF16) ? __bfloat16_as_ushort(__float2bfloat16_rn(out[j]))
+                                                  : __half_as_ushort(__float2half_rn(out[j]));
+    __syncwarp();
+    const int q8 = (lane & 3) * 8;
+    unsigned short* D = reinterpret_cast<unsigned short*>(p.D) + n0 + q8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = 8 * k + (lane >> 2);
+      if (row < left)
+        *reinterpret_cast<uint4*>(D + (r0 + static_cast<long long>(row)) * p.ldd) =
+            *reinterpret_cast<const uint4*>(&T[row * 32 + q8]);
+    }
+    __syncwarp();
+    return;
+  }
+  if (n < p.N) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) store_d(p.D, p.out_kind, (r0 + static_cast<long long>(j)) * p.ldd + n, out[j]);
+  }
+}
+
+// map_w: the weights (kExpF16: K-major boxes of 64 K x 128 N, or MN-major of
+// 64 N x 64 K; kExpMx4: 128 bytes x 128 rows). map_x / map_x64: the rows, in
+// boxes of BN and of 64 rows (a tile of few rows loads only what it needs).
+template <int KIND, int BN>
+__global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
+    experts_kernel(const __grid_constant__ CUtensorMap map_w,
+                   const __grid_constant__ CUtensorMap map_x,
+                   const __grid_constant__ CUtensorMap map_x64, const ExpertsParams p) {
+  using Cfg = ExpCfg<KIND, BN>;
+  constexpr int STAGES = Cfg::STAGES;
+  constexpr uint32_t SB = Cfg::STAGE_BYTES;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * SB);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* accf_bar = empty_bar + STAGES;  // [2]
+  uint64_t* acce_bar = accf_bar + 2;        // [2]
+  uint64_t* drain_bar = acce_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* epi = smem + STAGES * SB + 512;
+  GroupTable tb;
+  tb.row0 = reinterpret_cast<int*>(epi + kEpiStageBytes);
+  tb.tile0 = tb.row0 + kMaxGroups + 2;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const Abort ab{abort_flag, p.status, p.timeout_ns};
+
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1 + Cfg::SCALE_WARPS);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&accf_bar[a], 1);
+      mbar_init(&acce_bar[a], 4);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_x64);
+  }
+  if (warp == 0)
+    build_groups(tb, p.sizes, p.sizes64, p.groups, p.rows, BN, p.tiles_w, p.status);
+  __syncwarp();
+  if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
+  const int num_tiles = tb.tile0[p.groups + 1];
+  // tiles with products; the ones behind are stores of beta * C alone
+  const int work_tiles = num_kb ? tb.tile0[p.groups] : 0;
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool aborted = false;
+    for (int t = blockIdx.x; t < work_tiles && !aborted; t += gridDim.x) {
+      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+      // above three quarters of the tile one full box, else boxes of 64 rows
+      const int boxes = (BN == 64 || e.nv > BN * 3 / 4) ? 0 : (e.nv + 63) / 64;
+      const uint32_t bytes = Cfg::W_TILE + (boxes ? boxes * 64 * 128 : Cfg::X_TILE);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
+          aborted = true;
+          break;
+        }
+        uint8_t* sw = smem + stage * SB;
+        uint8_t* sx = sw + Cfg::W_TILE;
+        mbar_arrive_expect_tx(&full_bar[stage], bytes);
+        if constexpr (Cfg::MX) {
+          const int k0 = kb * 128;  // bytes
+          tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, e.g);
+          if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
+          for (int j = 0; j < boxes; ++j)
+            tma_load_3d(sx + j * 8192, &map_x64, &full_bar[stage], k0, e.r0 + 64 * j, 0);
+        } else {
+          const int k0 = kb * Cfg::BK;
+          const int gw = p.w_shared ? 0 : e.g;
+          if (!p.w_mn) {
+            tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, gw);
+          } else {
+            tma_load_3d(sw, &map_w, &full_bar[stage], e.n0, k0, gw);
+            tma_load_3d(sw + 8192, &map_w, &full_bar[stage], e.n0 + 64, k0, gw);
+          }
+          if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
+          for (int j = 0; j < boxes; ++j)
+            tma_load_3d(sx + j * 8192, &map_x64, &full_bar[stage], k0, e.r0 + 64 * j, 0);
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (aborted || ab.raised()) {
+      // let copies already issued land before the CTA exits (bounded)
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 20000000ull) {
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t sw0 = smem_u32(smem), sx0 = sw0 + Cfg::W_TILE;
+    uint64_t wd[4], xd[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      wd[kk] = (!Cfg::MX && p.w_mn) ? sdesc_sw128(sw0 + kk * 2048, 64 * 128, 1024)
+                                    : sdesc_sw128(sw0 + kk * 32, 16, 1024);
+      xd[kk] = sdesc_sw128(sx0 + kk * 32, 16, 1024);
+    }
+    const uint64_t sfd = sdesc_kmajor_noswz(sx0 + Cfg::X_TILE, 128, 128);
+    int stage = 0, tc = 0;
+    uint32_t phase = 0;
+    bool stop = false;
+    for (int t = blockIdx.x; t < work_tiles && !stop; t += gridDim.x, ++tc) {
+      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+      const uint32_t nm = static_cast<uint32_t>((e.nv + 15) & ~15);
+      const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn, 0, 128, nm);
+      const uint32_t id2 = idesc_mx4(nm, 2);
+      const int buf = tc & 1;
+      if (!mbar_wait(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + buf * BN;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, ab, kTimeoutFull)) {
+          stop = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t off = stage * SB;
+        if constexpr (Cfg::MX) {
+          const uint32_t sfw = tmem_base + 2 * BN + stage * Cfg::SF_COLS;
+          const uint32_t sfx = sfw + 8;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            tmem_cp_scales(sfw + 4 * w, sdesc_add(sfd, off + w * 512));
+#pragma unroll
+            for (int b = 0; b < Cfg::XBLK; ++b)
+              tmem_cp_scales(sfx + 4 * (w * Cfg::XBLK + b),
+                             sdesc_add(sfd, off + Cfg::SFW + (w * Cfg::XBLK + b) * 512));
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_mx4(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), (kk & 1) ? id2 : id,
+                    sfw + 4 * (kk >> 1), sfx + 4 * Cfg::XBLK * (kk >> 1), (kb | kk) ? 1u : 0u);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), id, (kb | kk) ? 1u : 0u);
+        }
+        tc_commit(&empty_bar[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!stop) tc_commit(&accf_bar[buf]);
+    }
+    // Every MMA this thread issued must finish before TMEM is released.
+    tc_commit(drain_bar);
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(drain_bar, 0)) {
+      if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
+        ab.raise(kTimeoutDrain);
+        break;
+      }
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;  // TMEM lane quarter
+    void* tsm = epi + (warp - 2) * (kEpiStageBytes / 4);
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
+    int tc = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+      const int n0 = e.n0 + 32 * q;
+      if (t >= work_tiles) {
+        float z[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = 0.0f;
+        if (n0 < p.N)
+          for (int c = 0; c < e.nv; c += 32) exp_store(p, e.r0 + c, min(32, e.nv - c), n0, z, tsm);
+        continue;
+      }
+      const int buf = tc & 1;
+      if (!mbar_wait_warp(&accf_bar[buf], (tc >> 1) & 1, ab, kTimeoutAccFull)) break;
+      ++tc;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < e.nv; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(lane_base + buf * BN + c, v);
+        tmem_ld_wait();
+        if (n0 < p.N) {
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = u2f(v[j]);
+          exp_store(p, e.r0 + c, min(32, e.nv - c), n0, f, tsm);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acce_bar[buf]);
+    }
+  } else if (Cfg::MX && warp >= 6) {
+    // ------------------------------------------------------------ scales
+    // Warp 6 + w brings scale word w of every stage (K = 128), two stages in
+    // flight behind the one being asked for.
+    const int w = warp - 6;
+    const int kwords = (p.K + 127) / 128;
+    const uint32_t s0 = smem_u32(smem) + Cfg::W_TILE + Cfg::X_TILE;
+    int stage = 0, sig = 0, pending = 0;
+    uint32_t phase = 0;
+    bool stop = false;
+    auto signal = [&] {
+      fence_proxy_async_smem();  // tcgen05.cp reads what the copies wrote
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full_bar[sig]);
+      if (++sig == STAGES) sig = 0;
+      --pending;
+    };
+    for (int t = blockIdx.x; t < work_tiles && !stop; t += gridDim.x) {
+      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+      const uint32_t* wrow = p.ws + static_cast<long long>(e.g) * p.N + e.n0;
+      const uint32_t* xrow = p.xs + e.r0;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1u, ab, kTimeoutAux)) {
+          stop = true;
+          break;
+        }
+        const int kw = kb * 2 + w;
+        const bool kok = kw < kwords;
+        const uint32_t dst = s0 + stage * SB + lane * 16;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int i = lane + 32 * c;
+          const bool ok = kok && e.n0 + i < p.N;
+          cp_async4(dst + w * 512 + 4 * c, ok ? wrow + static_cast<long long>(kw) * p.ws_rows + i : p.ws, ok);
+        }
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          const int i = lane + 32 * c;
+          const bool ok = kok && i < e.nv;
+          cp_async4(dst + Cfg::SFW + w * Cfg::XBLK * 512 + (c >> 2) * 512 + (c & 3) * 4,
+                    ok ? xrow + static_cast<long long>(kw) * p.xs_rows + i : p.xs, ok);
+        }
+        cp_async_commit();
+        if (++pending > 2) {
+          cp_async_wait<2>();
+          signal();
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    cp_async_wait<0>();
+    while (pending) signal();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace tb

@@ -1,0 +1,261 @@
+// Weight gradient of the products grouped by expert (a ragged contraction).
+#pragma once
+
+#include "experts_sm100.cuh"
+
+namespace tb {
+
+// ---------------------------------------------------------------------------
+// Weight gradient: D[g] (M x N) = alpha * A_g^T B_g + beta * C[g], A_g the
+// group's rows of A (rows x M), B_g of B (rows x N), both read MN-major in
+// boxes of 64 columns x 64 rows. The contraction runs over a group's rows, so
+// its last block reaches into the next group: a fixer warp overwrites those
+// rows with zeros in shared memory (both operands: a zero times an infinity of
+// another group would be a NaN) before the MMAs of the stage, which run only
+// the 16-row steps that hold rows of the group. A group without rows stores
+// beta * C.
+// ---------------------------------------------------------------------------
+struct WgradParams {
+  GemmParams p;  // M, N, alpha, beta, C, D, out_kind, c_mode, status, timeout
+  int rows, groups;
+  const void* sizes;
+  int sizes64;
+  int in_fmt;
+};
+
+struct WgradCfg {
+  static constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4;
+  static constexpr int A_TILE = BM * 128, B_TILE = BN * 128;
+  static constexpr int STAGE_BYTES = A_TILE + B_TILE;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int THREADS = 32 * 7;  // producer, MMA, 4 epilogue, fixer
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + (kMaxGroups + 2) * 4;
+};
+
+__global__ void __launch_bounds__(WgradCfg::THREADS, 1)
+    wgrad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const WgradParams w) {
+  using Cfg = WgradCfg;
+  constexpr int STAGES = Cfg::STAGES;
+  constexpr uint32_t SB = Cfg::STAGE_BYTES;
+  const GemmParams& p = w.p;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * SB);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* fix_bar = empty_bar + STAGES;  // the stage's rows behind the group are zero
+  uint64_t* accf_bar = fix_bar + STAGES;   // [2]
+  uint64_t* acce_bar = accf_bar + 2;       // [2]
+  uint64_t* drain_bar = acce_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  GroupTable tb;
+  tb.row0 = reinterpret_cast<int*>(smem + STAGES * SB + 512);
+  tb.tile0 = nullptr;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const Abort ab{abort_flag, p.status, p.timeout_ns};
+
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+      mbar_init(&fix_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&accf_bar[a], 1);
+      mbar_init(&acce_bar[a], 4);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 0) build_groups(tb, w.sizes, w.sizes64, w.groups, w.rows, 0, 0, p.status);
+  __syncwarp();
+  if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int per_group = p.tiles_m * p.tiles_n;
+  struct Tile {
+    int g, m0, n0, r0, m;
+  };
+  auto tile = [&](int t) -> Tile {
+    Tile e;
+    e.g = t / per_group;
+    const int i = t - e.g * per_group;
+    e.m0 = (i % p.tiles_m) * Cfg::BM;
+    e.n0 = (i / p.tiles_m) * Cfg::BN;
+    e.r0 = tb.row0[e.g];
+    e.m = tb.row0[e.g + 1] - e.r0;
+    return e;
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool aborted = false;
+    for (int t = blockIdx.x; t < p.num_tiles && !aborted; t += gridDim.x) {
+      const Tile e = tile(t);
+      for (int r = 0; r < e.m; r += Cfg::BK) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
+          aborted = true;
+          break;
+        }
+        uint8_t* sa = smem + stage * SB;
+        uint8_t* sb = sa + Cfg::A_TILE;
+        mbar_arrive_expect_tx(&full_bar[stage], SB);
+#pragma unroll
+        for (int j = 0; j < Cfg::BM / 64; ++j)
+          tma_load_3d(sa + j * 8192, &map_a, &full_bar[stage], e.m0 + 64 * j, e.r0 + r, 0);
+#pragma unroll
+        for (int j = 0; j < Cfg::BN / 64; ++j)
+          tma_load_3d(sb + j * 8192, &map_b, &full_bar[stage], e.n0 + 64 * j, e.r0 + r, 0);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (aborted || ab.raised()) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 20000000ull) {
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t id = idesc(kAccF32, w.in_fmt, w.in_fmt, 1, 1, Cfg::BM, Cfg::BN);
+    const uint32_t sa0 = smem_u32(smem), sb0 = sa0 + Cfg::A_TILE;
+    uint64_t ad[4], bd[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      ad[kk] = sdesc_sw128(sa0 + kk * 2048, 64 * 128, 1024);
+      bd[kk] = sdesc_sw128(sb0 + kk * 2048, 64 * 128, 1024);
+    }
+    int stage = 0, tc = 0;
+    uint32_t phase = 0;
+    bool stop = false;
+    for (int t = blockIdx.x; t < p.num_tiles && !stop; t += gridDim.x) {
+      const Tile e = tile(t);
+      if (e.m == 0) continue;
+      const int buf = tc & 1;
+      if (!mbar_wait(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
+      ++tc;
+      tc_fence_after();
+      const uint32_t d = tmem_base + buf * Cfg::BN;
+      for (int r = 0; r < e.m; r += Cfg::BK) {
+        if (!mbar_wait(&fix_bar[stage], phase, ab, kTimeoutFull)) {
+          stop = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t off = stage * SB;
+        const int steps = min(4, (e.m - r + 15) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (kk < steps)
+            mma_f16(d, sdesc_add(ad[kk], off), sdesc_add(bd[kk], off), id, (r | kk) ? 1u : 0u);
+        tc_commit(&empty_bar[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!stop) tc_commit(&accf_bar[buf]);
+    }
+    tc_commit(drain_bar);
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(drain_bar, 0)) {
+      if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
+        ab.raise(kTimeoutDrain);
+        break;
+      }
+    }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------ fixer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool stop = false;
+    for (int t = blockIdx.x; t < p.num_tiles && !stop; t += gridDim.x) {
+      const Tile e = tile(t);
+      for (int r = 0; r < e.m; r += Cfg::BK) {
+        if (!mbar_wait_warp(&full_bar[stage], phase, ab, kTimeoutAux)) {
+          stop = true;
+          break;
+        }
+        const int v = e.m - r;  // rows of the group in this block
+        if (v < Cfg::BK && (v & 15)) {
+          // rows v .. round_up(v, 16) of each box, 128 bytes each (the swizzle
+          // permutes 16-byte pieces within a row)
+          const int pieces = (16 - (v & 15)) * 8;
+          for (int b = 0; b < (Cfg::BM + Cfg::BN) / 64; ++b) {
+            uint4* z = reinterpret_cast<uint4*>(smem + stage * SB + b * 8192 + v * 128);
+            for (int i = lane; i < pieces; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&fix_bar[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
+    int tc = 0;
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
+      const Tile e = tile(t);
+      const int r = e.m0 + 32 * q + lane;
+      const int buf = tc & 1;
+      if (e.m) {
+        if (!mbar_wait_warp(&accf_bar[buf], (tc >> 1) & 1, ab, kTimeoutAccFull)) break;
+        ++tc;
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int c = 0; c < Cfg::BN / 32; ++c) {
+        uint32_t v[32];
+        if (e.m) {
+          tmem_ld32(lane_base + buf * Cfg::BN + c * 32, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0;
+        }
+        if (e.n0 + c * 32 < p.N) {
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = u2f(v[j]);
+          epilogue_row32(p, e.g, r, e.n0 + c * 32, f);
+        }
+      }
+      if (e.m) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acce_bar[buf]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace tb

@@ -44,6 +44,21 @@ bool load_encode() {
   g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   return true;
 }
+
+// Encode a tensor map. A thread that has made no CUDA runtime call yet (an
+// autograd worker's first backward) has no current context, which the driver
+// call needs: cudaSetDevice makes the device's primary context current.
+CUresult encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank, void* base,
+                      const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                      const cuuint32_t* estr, CUtensorMapSwizzle swizzle) {
+  auto call = [&] {
+    return g_encode(map, dt, rank, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = call();
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaSetDevice(current_device()) == cudaSuccess) r = call();
+  return r;
+}
 }  // namespace
 
 void set_error(const std::string& msg) { g_last_error = msg; }
@@ -150,9 +165,8 @@ bool encode_map_3d(CUtensorMap* map, CUtensorMapDataType dt, int esize, const vo
   cuuint64_t strides[2] = {s1b, s2b};
   cuuint32_t box[3] = {box0, box1, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
     return false;
@@ -203,9 +217,8 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType dt, int esize, const void*
     }
     st[i] = b;
   }
-  CUresult r = g_encode(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st,
-                        bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
+                                  d, st, bx, es, swizzle);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
     return false;

@@ -1,0 +1,239 @@
+"""Products grouped by expert: `grouped_gemm` and the gradient of its weights,
+`grouped_gemm_wgrad`.
+
+The rows of one operand fall into groups of any length (the tokens a router
+sent to each expert), and every group has its own matrix. They stand beside
+`batched_gemm`, whose entries all have one size; the reference has no
+counterpart. The sizes stay on the device: no call synchronises with the host,
+and a captured graph follows the sizes of each replay. bfloat16 and float16 on
+the sm_100a kernels through the C ABI; other dtypes raise TypeError.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _native as N
+from ._flags import trans_flag
+from .level3 import _add_c, _cuda_device, _flat_batch, _fuse_c, _home, _mixed_dtype_error, _tma_operand, _to
+
+DTYPES = (torch.bfloat16, torch.float16)
+MAX_GROUPS = 1024
+
+
+def _on(dev: torch.device):
+    """The operands' device current, for a call made with another one current."""
+    if dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _check_types(name: str, a, b, out_dtype):
+    for x in (a, b):
+        if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES:
+            raise TypeError(f"{name}: operands are bfloat16 or float16 tensors, got {getattr(x, 'dtype', type(x))}")
+    if a.dtype != b.dtype:
+        _mixed_dtype_error(a, b)
+    out = a.dtype if out_dtype is None else out_dtype
+    if out not in (a.dtype, torch.float32):
+        raise TypeError(f"{name}: out_dtype is {a.dtype} or float32, got {out_dtype}")
+    return out
+
+
+def check_group_sizes(name: str, sizes, groups: int | None, rows: int) -> None:
+    """Shape and dtype of the sizes; their values only where the host holds them."""
+    if not isinstance(sizes, torch.Tensor) or sizes.dim() != 1 or sizes.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: group_sizes is a 1-D int32 or int64 tensor")
+    if groups is not None and sizes.shape[0] != groups:
+        raise ValueError(f"{name}: {sizes.shape[0]} group sizes for {groups} matrices")
+    if sizes.shape[0] > MAX_GROUPS:
+        raise ValueError(f"{name}: at most {MAX_GROUPS} groups, got {sizes.shape[0]}")
+    if sizes.device.type == "cpu" and sizes.numel():
+        if int(sizes.min()) < 0 or int(sizes.sum()) > rows:
+            raise ValueError(f"{name}: group sizes must not be negative nor sum to more than the {rows} rows")
+
+
+def _rows_operand(x: torch.Tensor):
+    """(tensor, ld) of a rows x cols operand stored row by row on 16 bytes."""
+    t, ld, tr = _tma_operand(x, x.element_size())
+    if tr:
+        t, ld, tr = _tma_operand(x.contiguous(), x.element_size())
+    if tr:  # a single column: pad its rows
+        q = 16 // x.element_size()
+        t = x.new_zeros((x.shape[0], q))
+        t[:, : x.shape[1]].copy_(x)
+        ld = q
+    return t, ld
+
+
+def _c_operand(C, cols: int):
+    """(tensor, ld) of a 2-D C whose rows are contiguous."""
+    c = C if C.stride(-1) == 1 and C.stride(-2) >= cols else C.contiguous()
+    return c, c.stride(-2)
+
+
+def _grouped(alpha, a, b, sizes, beta, C, out_dtype):
+    """alpha * a[r] @ b[g] (+ beta * C) on the kernel; C fusable or None."""
+    rows, K = a.shape
+    G, _, Nn = b.shape
+    dev = a.device
+    out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
+    if rows == 0 or Nn == 0:
+        return out
+    at, lda, bt, ldb, tb, sb = a, K, b, Nn, False, 0
+    if K and G:
+        at, lda = _rows_operand(a)
+        bt, ldb, tb, sb = _flat_batch(b, (G,), b.element_size(), False)
+    c_arg, ldc = _c_operand(C, Nn) if C is not None else (None, 0)
+    sizes = sizes.contiguous()
+    with _on(dev):
+        rc = N.lib().trnblas_grouped_gemm(
+            N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(at), lda,
+            N.ptr(bt), ldb, sb, int(tb), N.ptr(sizes), int(sizes.dtype == torch.int64),
+            float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, N.ptr(out), Nn, N.stream_ptr(dev))
+    N.check(rc, "trnblas_grouped_gemm")
+    N.count_launches(1)
+    return out
+
+
+def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
+    """alpha * a_g^T @ b_g (+ beta * C[g]) on the kernel; C fusable or None."""
+    rows, M = a.shape
+    Nn = b.shape[1]
+    G = sizes.shape[0]
+    dev = a.device
+    out = torch.empty((G, M, Nn), dtype=out_dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    (at, lda), (bt, ldb) = (_rows_operand(a), _rows_operand(b)) if rows else ((a, M), (b, Nn))
+    c_arg, ldc, sc = None, 0, 0
+    if C is not None:
+        c_arg, ldc = _c_operand(C, Nn)
+        sc = c_arg.stride(0)
+    sizes = sizes.contiguous()
+    with _on(dev):
+        rc = N.lib().trnblas_grouped_gemm_wgrad(
+            N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, M, Nn, float(alpha), N.ptr(at), lda,
+            N.ptr(bt), ldb, N.ptr(sizes), int(sizes.dtype == torch.int64),
+            float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, sc, N.ptr(out), Nn, M * Nn, N.stream_ptr(dev))
+    N.check(rc, "trnblas_grouped_gemm_wgrad")
+    N.count_launches(1)
+    return out
+
+
+class _GroupedGemm(torch.autograd.Function):
+    """D[r] = alpha A[r] b[g] + beta C[r] with its gradients:
+    dA[r] = alpha dD[r] b[g]^T, db[g] = alpha A_g^T dD_g, dC = beta dD."""
+
+    @staticmethod
+    def forward(ctx, alpha, a, b, sizes, beta, C, out_dtype):
+        ctx.save_for_backward(a, b, sizes)
+        ctx.factors = (alpha, beta)
+        return _grouped(alpha, a, b, sizes, beta, C, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dD):
+        a, b, sizes = ctx.saved_tensors
+        alpha, beta = ctx.factors
+        y = dD.to(a.dtype)
+        da = db = dC = None
+        if ctx.needs_input_grad[1]:
+            da = _grouped(alpha, y, b.mT, sizes, 0.0, None, a.dtype)
+        if ctx.needs_input_grad[2]:
+            # in the layout of b's storage: b may be the transpose of what the caller holds
+            if b.stride(-2) == 1 and b.stride(-1) != 1:
+                db = _wgrad(alpha, y, a, sizes, 0.0, None, b.dtype).mT
+            else:
+                db = _wgrad(alpha, a, y, sizes, 0.0, None, b.dtype)
+        if ctx.needs_input_grad[5]:
+            dC = beta * dD
+        return None, da, db, None, None, dC, None
+
+
+def grouped_gemm(
+    alpha: float,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    group_sizes: torch.Tensor,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+    transB: bool = False,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """D[r] = alpha * A[r] @ op(B[g]) + beta * C[r] for the rows r of group g.
+
+    A is (rows, K); its first group_sizes[0] rows belong to group 0, the next
+    group_sizes[1] to group 1, and so on. B is (G, K, N), or (G, N, K) with
+    transB; it may be expanded (one matrix for all groups). Rows behind the last
+    group are an empty product: beta * C[r], or zero. group_sizes is int32 or
+    int64 on any device; on the host its values are checked (ValueError), on
+    the device negative sizes count as zero, sizes beyond the rows are cut
+    off, and `device_status` then returns 8. At most 1024 groups. bfloat16 or
+    float16 with fp32 accumulation; the result (rows, N) has the operands'
+    dtype or float32 (out_dtype). alpha, beta and a same-shape C of the result's
+    dtype are fused; another C is added afterwards with torch semantics.
+
+    Differentiable in A, B and C (once): the gradients run on the same kernels,
+    rounded once to their operand's dtype. Inside a CUDA graph capture, call
+    `grouped_gemm` (transB flipped) and `grouped_gemm_wgrad` for them directly,
+    or capture forward and backward together on leaves used on no other stream.
+    """
+    name = "grouped_gemm"
+    transB = trans_flag(transB, "transB")
+    out_dtype = _check_types(name, A, B, out_dtype)
+    if A.dim() != 2 or B.dim() != 3:
+        raise ValueError(f"{name}: A is 2-D and B 3-D, got {tuple(A.shape)} and {tuple(B.shape)}")
+    b = B.mT if transB else B
+    if A.shape[1] != b.shape[1]:
+        raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, op(B) {tuple(b.shape)}")
+    check_group_sizes(name, group_sizes, b.shape[0], A.shape[0])
+    home = A.device
+    dev = _cuda_device(A, B, C, group_sizes)
+    a, b, sizes, Cd = _to(A, dev), _to(b, dev), _to(group_sizes, dev), _to(C, dev)
+    fuse = _fuse_c(Cd, beta, (a.shape[0], b.shape[2]), out_dtype, dev)
+    c_arg = Cd if fuse else None
+    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or (fuse and Cd.requires_grad)):
+        r = _GroupedGemm.apply(alpha, a, b, sizes, beta, c_arg, out_dtype)
+        if not fuse and C is not None and beta != 0.0:
+            r = r + beta * Cd
+        return r if home == dev else r.to(home)
+    r = _grouped(alpha, a, b, sizes, beta, c_arg, out_dtype)
+    if not fuse:
+        r = _add_c(r, beta, Cd)
+    return _home(r, home, dev)
+
+
+def grouped_gemm_wgrad(
+    alpha: float,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    group_sizes: torch.Tensor,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """D[g] = alpha * A_g^T @ B_g + beta * C[g], the contraction over the rows
+    of group g: for A the operand and B the result's gradient of `grouped_gemm`,
+    the gradient of its (G, K, N) weights; with A and B exchanged that of
+    (G, N, K) weights. C (G, M, N) of the result's dtype adds to a running
+    gradient (beta = 1, out_dtype = float32 keeps it in 32 bits). A group
+    without rows gives beta * C[g]. Rows behind the last group are not part of
+    any sum. group_sizes and dtypes as for `grouped_gemm`; not differentiable.
+    """
+    name = "grouped_gemm_wgrad"
+    out_dtype = _check_types(name, A, B, out_dtype)
+    if A.dim() != 2 or B.dim() != 2 or A.shape[0] != B.shape[0]:
+        raise ValueError(f"{name}: A and B are 2-D with the same rows, got {tuple(A.shape)} and {tuple(B.shape)}")
+    check_group_sizes(name, group_sizes, None, A.shape[0])
+    home = A.device
+    dev = _cuda_device(A, B, C, group_sizes)
+    a, b, sizes, Cd = (_to(A.detach(), dev), _to(B.detach(), dev), _to(group_sizes, dev),
+                       _to(C.detach() if isinstance(C, torch.Tensor) else C, dev))
+    fuse = _fuse_c(Cd, beta, (sizes.shape[0], a.shape[1], b.shape[1]), out_dtype, dev)
+    r = _wgrad(alpha, a, b, sizes, beta, Cd if fuse else None, out_dtype)
+    if not fuse:
+        r = _add_c(r, beta, Cd)
+    return _home(r, home, dev)
