@@ -286,33 +286,53 @@ TRNBLAS_API int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t row
 /*
  * Microscaled 4-bit floating point (OCP MX, MXFP4): blocks of 32 values along
  * K, each value E2M1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), each
- * block with a power of two 2^(s - 127), s one byte. `data` holds two values a
- * byte, the even one in the low half, rows ldq bytes apart (a multiple of 16,
- * at least round_up(K, 32) / 2; K is padded with zeros); `scales` holds one
- * 4-byte word for every row and 128 values of K, at [k / 128][row].
+ * block with a power of two 2^(s - 127), s one byte. A stack of `matrices`
+ * matrices of rows x K (X, row stride ldx in elements, F32, BF16 or F16):
+ * `data` holds two values a byte, the even one in the low half, all rows ldq
+ * bytes apart (a multiple of 16, at least round_up(K, 32) / 2; K is padded
+ * with zeros). `scales` holds 512 bytes for every 128 rows of a matrix and
+ * every 128 values of K, [matrix][row / 128][k / 128]: the four bytes of row r
+ * at 16 * (r % 32) + 4 * (r / 32 % 4), zero past the rows and past K. Both on
+ * 16 bytes.
  * s is the biased exponent of the block's largest magnitude less 2 (at least
  * 0); values round to nearest, ties to the even mantissa, and saturate at 6.
- * A block with an infinity or a NaN becomes s = 255: all NaN. X is F32, BF16
- * or F16, rows x K, row stride ldx. trnblas_mxfp4_dequantize gives the values
- * back in F32, BF16 or F16. No counterpart in the reference.
+ * A block with an infinity or a NaN becomes s = 255: all NaN.
+ * trnblas_mxfp4_dequantize gives the values back in F32, BF16 or F16. No
+ * counterpart in the reference.
  */
-TRNBLAS_API int trnblas_mxfp4_quantize(int dtype, int64_t rows, int64_t K, const void* X, int64_t ldx,
-                           void* data, int64_t ldq, void* scales, void* stream);
-TRNBLAS_API int trnblas_mxfp4_dequantize(int dtype, int64_t rows, int64_t K, const void* data, int64_t ldq,
-                             const void* scales, void* Y, int64_t ldy, void* stream);
+TRNBLAS_API int trnblas_mxfp4_quantize(int dtype, int64_t matrices, int64_t rows, int64_t K, const void* X,
+                           int64_t ldx, void* data, int64_t ldq, void* scales, void* stream);
+TRNBLAS_API int trnblas_mxfp4_dequantize(int dtype, int64_t matrices, int64_t rows, int64_t K,
+                             const void* data, int64_t ldq, const void* scales, void* Y,
+                             int64_t ldy, void* stream);
 
 /*
  * D[r] = alpha * A[r] @ B[g]^T + beta * C[r] on block-scaled 4-bit tensor
- * cores, fp32 accumulate: A (rows x K) and B (`groups` stacked N x K matrices,
- * quantised as one operand of groups * N rows) as trnblas_mxfp4_quantize
- * writes them (lda, ldb in bytes), C and D rows x N of out_dtype (F32, BF16 or
- * F16). group_sizes as for trnblas_grouped_gemm; NULL with groups = 1 is the
- * dense product. No counterpart in the reference.
+ * cores, fp32 accumulate: A (one matrix, rows x K) and B (`groups` matrices of
+ * N x K) as trnblas_mxfp4_quantize writes them (lda, ldb in bytes), C and D
+ * rows x N of out_dtype (F32, BF16 or F16). group_sizes as for
+ * trnblas_grouped_gemm; NULL with groups = 1 is the dense product, which needs
+ * no workspace. A grouped one brings A's scales into blocks that start with the
+ * groups first (workspace, 16-byte aligned). No counterpart in the reference.
  */
+TRNBLAS_API size_t trnblas_mxfp4_gemm_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped);
 TRNBLAS_API int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K,
                        float alpha, const void* A, int64_t lda, const void* scalesA, const void* B,
                        int64_t ldb, const void* scalesB, const void* group_sizes, int sizes_64,
-                       float beta, const void* C, int64_t ldc, void* D, int64_t ldd, void* stream);
+                       float beta, const void* C, int64_t ldc, void* D, int64_t ldd,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * trnblas_mxfp4_gemm on rows X (F32, BF16 or F16, row stride ldx in elements)
+ * that are quantised on the way, as trnblas_mxfp4_quantize does, into the
+ * workspace (16-byte aligned).
+ */
+TRNBLAS_API size_t trnblas_mxfp4_gemm_x_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped);
+TRNBLAS_API int trnblas_mxfp4_gemm_x(int a_dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N,
+                         int64_t K, float alpha, const void* X, int64_t ldx, const void* B,
+                         int64_t ldb, const void* scalesB, const void* group_sizes, int sizes_64,
+                         float beta, const void* C, int64_t ldc, void* D, int64_t ldd,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Self-test of the bounded-wait machinery: launches one CTA that waits on an

@@ -20,7 +20,7 @@ def _mx(*shape):
     for n in lead:
         rows *= n
     return tb.MXFP4Tensor(torch.zeros(*lead, -(-K // 32) * 16, dtype=torch.uint8),
-                          torch.zeros(-(-K // 128), rows, 4, dtype=torch.uint8), shape)
+                          torch.zeros(rows // lead[-1], -(-lead[-1] // 128), -(-K // 128), 512, dtype=torch.uint8), shape)
 
 
 @pytest.mark.parametrize("call,exc", [
@@ -54,9 +54,9 @@ def _mx(*shape):
     (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(3, 8), S), ValueError),
     (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), torch.tensor([6, 1])), ValueError),
     (lambda: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), torch.tensor([6])), ValueError),
-    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(1, 3, 4, dtype=torch.uint8), (3, 33)), ValueError),
-    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16), torch.zeros(1, 3, 4, dtype=torch.uint8), (3, 32)), ValueError),
-    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(2, 3, 4, dtype=torch.uint8), (3, 32)), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(1, 1, 1, 512, dtype=torch.uint8), (3, 33)), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16), torch.zeros(1, 1, 1, 512, dtype=torch.uint8), (3, 32)), ValueError),
+    (lambda: tb.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(1, 1, 2, 512, dtype=torch.uint8), (3, 32)), ValueError),
     (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 16), torch.zeros(3, 1, dtype=torch.uint8), 32), TypeError),
     (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 15, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 32), ValueError),
     (lambda: tb.MXFP4Tensor.from_parts(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 2, dtype=torch.uint8), 32), ValueError),
@@ -100,20 +100,34 @@ def test_c_entry_points_check_their_arguments():
                  (N.F32, 4, 8, FAKE, 7, FAKE, 16, FAKE), (N.F32, 4, 8, FAKE, 8, FAKE, 8, FAKE),
                  (N.F32, 4, 33, FAKE, 33, FAKE, 16, FAKE), (N.F32, 4, 8, None, 8, FAKE, 16, FAKE),
                  (N.F32, 4, 8, FAKE, 8, FAKE + 8, 16, FAKE), (N.F32, 4, 8, FAKE, 8, FAKE, 16, FAKE + 2)):
-        assert q(*args, None) == N.ERR_ARG, args
+        assert q(args[0], 1, *args[1:], None) == N.ERR_ARG, args
+    assert q(N.F32, -1, 4, 8, FAKE, 8, FAKE, 16, FAKE, None) == N.ERR_ARG
     dq = L.trnblas_mxfp4_dequantize
     for args in ((N.F64, 4, 8, FAKE, 16, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, FAKE, FAKE, 7),
                  (N.F32, 4, 8, FAKE, 15, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, None, FAKE, 8)):
-        assert dq(*args, None) == N.ERR_ARG, args
+        assert dq(args[0], 1, *args[1:], None) == N.ERR_ARG, args
 
     def mx(od=N.BF16, rows=4, G=1, n=8, k=64, a=FAKE, lda=32, sa=FAKE, b=FAKE, ldb=32, sb=FAKE, s=None, c=None, ldc=0,
            d=FAKE, ldd=8):
-        return L.trnblas_mxfp4_gemm(od, rows, G, n, k, 1.0, a, lda, sa, b, ldb, sb, s, 0, 1.0, c, ldc, d, ldd, None)
+        return L.trnblas_mxfp4_gemm(od, rows, G, n, k, 1.0, a, lda, sa, b, ldb, sb, s, 0, 1.0, c, ldc, d, ldd, None, 0, None)
 
     for bad in (dict(od=N.F64), dict(rows=-1), dict(G=2), dict(G=1025, s=FAKE), dict(d=None), dict(ldd=7), dict(lda=16),
                 dict(ldb=31), dict(a=None), dict(sa=FAKE + 1), dict(sb=None), dict(c=FAKE, ldc=7)):
         assert mx(**bad) == N.ERR_ARG, bad
     assert mx(rows=0) == 0
+    assert mx(s=FAKE) == N.ERR_WORKSPACE  # grouped: the scale blocks need a workspace
+    assert L.trnblas_mxfp4_gemm_workspace_size(300, 2, 200, 1) == (3 + 2) * 2 * 512
+    assert L.trnblas_mxfp4_gemm_workspace_size(300, 1, 200, 0) == 0
+    assert L.trnblas_mxfp4_gemm_x_workspace_size(300, 2, 200, 1) == 300 * 112 + 5 * 2 * 512
+
+    def gx(dt=N.BF16, ws=FAKE, n=1 << 20, x=FAKE, ldx=64):
+        return L.trnblas_mxfp4_gemm_x(dt, N.BF16, 4, 1, 8, 64, 1.0, x, ldx, FAKE, 32, FAKE, None, 0, 0.0, None, 0, FAKE, 8,
+                                      ws, n, None)
+
+    for bad in (dict(dt=N.F64), dict(x=None), dict(ldx=63)):
+        assert gx(**bad) == N.ERR_ARG, bad
+    for bad in (dict(ws=None), dict(ws=FAKE + 8), dict(n=4 * 32 + 511)):
+        assert gx(**bad) == N.ERR_WORKSPACE, bad
 
 
 @pytest.mark.parametrize("K", [1, 2, 31, 32, 33, 64, 127, 128, 129, 300])
@@ -130,12 +144,30 @@ def test_parts_round_trip(K):
     if K % 2:
         want[..., -1] &= 0x0F
     assert torch.equal(c[..., : want.shape[-1]], want) and (c[..., want.shape[-1]:] == 0).all()
-    # word [k / 128][row] holds the row's four blocks there
-    words = q.scales
-    for r in range(10):
-        for b in range(4 * words.shape[0]):
-            v = words[b // 4, r, b % 4]
-            assert v == (scales.view(10, nb)[r, b] if b < nb else 0)
+    # byte [matrix][row / 128][k / 128][16 (r % 32) + 4 (r / 32 % 4) + block % 4]
+    f = q.scales
+    seen = torch.zeros_like(f, dtype=torch.bool)
+    for m in range(2):
+        for r in range(5):
+            for b in range(nb):
+                at = (m, r // 128, b // 4, 16 * (r % 32) + 4 * (r // 32 % 4) + b % 4)
+                assert f[at] == scales[m, r, b]
+                seen[at] = True
+    assert (f[~seen] == 0).all()
+
+
+def test_parts_of_many_rows():
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randint(0, 256, (300, 80), dtype=torch.uint8, generator=g)
+    scales = torch.randint(0, 256, (300, 5), dtype=torch.uint8, generator=g)
+    q = tb.MXFP4Tensor.from_parts(codes, scales, 160)
+    assert q.scales.shape == (1, 3, 2, 512)
+    for r in (0, 31, 32, 127, 128, 200, 299):
+        for b in range(5):
+            assert q.scales[0, r // 128, b // 4, 16 * (r % 32) + 4 * (r // 32 % 4) + b % 4] == scales[r, b]
+    c, s = q.parts()
+    assert torch.equal(c, codes) and torch.equal(s, scales)
+    assert tb.MXFP4Tensor.from_parts(codes[:0], scales[:0], 160).parts()[1].shape == (0, 5)
 
 
 def test_oracle_quantiser_by_hand():

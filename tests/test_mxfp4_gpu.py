@@ -56,8 +56,8 @@ def test_quantise_bit_for_bit(dt, rows, K):
     assert torch.equal(tb.dequantize_mxfp4(q).double(), ref)
     assert torch.equal(tb.dequantize_mxfp4(q, BF).double(), ref)
     assert torch.equal(tb.dequantize_mxfp4(q, FP), ref.to(F32).to(FP))
-    words = q.scales.transpose(0, 1).reshape(rows, -1)
-    assert (words[:, -(-K // 32):] == 0).all() and (codes[:, -(-K // 2):] == 0).all()
+    again = tb.MXFP4Tensor.from_parts(codes, scales, K)  # zeros behind the rows and behind K
+    assert torch.equal(again.scales, q.scales) and torch.equal(again.data, q.data)
 
 
 def test_every_float_of_a_grid_and_the_extremes():
@@ -99,7 +99,8 @@ def test_quantise_layouts():
     assert torch.equal(tb.quantize_mxfp4(part).data, want.data)
     y = _rand(3, 7, 160)
     q3, q2 = tb.quantize_mxfp4(y), tb.quantize_mxfp4(y.reshape(21, 160))
-    assert q3.shape == (3, 7, 160) and torch.equal(q3.scales, q2.scales) and torch.equal(q3.data.view(21, -1), q2.data)
+    assert q3.shape == (3, 7, 160) and torch.equal(q3.data.view(21, -1), q2.data)
+    assert torch.equal(q3.parts()[1].view(21, -1), q2.parts()[1])
     qc = tb.quantize_mxfp4(y.cpu())
     assert qc.device.type == "cpu" and torch.equal(qc.data, q3.data.cpu())
     assert torch.equal(tb.dequantize_mxfp4(qc), tb.dequantize_mxfp4(q3).cpu())
@@ -107,7 +108,7 @@ def test_quantise_layouts():
 
 
 DENSE = [(1, 128, 64), (1, 8, 32), (3, 130, 33), (17, 257, 256), (64, 128, 1000), (65, 384, 128), (200, 100, 520),
-         (192, 256, 256), (385, 200, 4096), (1000, 640, 776)]
+         (192, 256, 256), (385, 200, 4096), (1000, 640, 776), (448, 129, 288), (321, 300, 640)]
 
 
 @pytest.mark.parametrize("M,Nn,K", DENSE)
@@ -160,7 +161,7 @@ def test_alpha_beta_c_and_nan_scales():
     assert tb.gemm_mxfp4(1.0, _rand(0, 64), tb.quantize_mxfp4(_rand(7, 64))).shape == (0, 7)
 
 
-SIZES = [[0], [1], [0, 0, 5, 0], [300, 0, 1, 17], [64, 65, 63, 1, 0, 128], [193, 192, 191, 400], [2] * 37]
+SIZES = [[0], [1], [0, 0, 5, 0], [300, 0, 1, 17], [64, 65, 63, 1, 0, 128], [193, 192, 191, 400], [2] * 37, [130, 257, 0, 385, 63]]
 
 
 @pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")

@@ -79,10 +79,17 @@ _SIGNATURES = {
         _i,
         [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p, _i, _f, _p, _i64, _i64, _p, _i64, _i64, _p],
     ),
-    "trnblas_mxfp4_quantize": (_i, [_i, _i64, _i64, _p, _i64, _p, _i64, _p, _p]),
-    "trnblas_mxfp4_dequantize": (_i, [_i, _i64, _i64, _p, _i64, _p, _p, _i64, _p]),
+    "trnblas_mxfp4_quantize": (_i, [_i, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p]),
+    "trnblas_mxfp4_dequantize": (_i, [_i, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p]),
+    "trnblas_mxfp4_gemm_workspace_size": (_sz, [_i64, _i64, _i64, _i]),
     "trnblas_mxfp4_gemm": (
-        _i, [_i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _p, _i64, _p, _p, _i, _f, _p, _i64, _p, _i64, _p]
+        _i,
+        [_i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _p, _i64, _p, _p, _i, _f, _p, _i64, _p, _i64, _p, _sz, _p],
+    ),
+    "trnblas_mxfp4_gemm_x_workspace_size": (_sz, [_i64, _i64, _i64, _i]),
+    "trnblas_mxfp4_gemm_x": (
+        _i,
+        [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p, _p, _i, _f, _p, _i64, _p, _i64, _p, _sz, _p],
     ),
     "trnblas_wait_selftest": (_i, [ctypes.c_ulonglong, _p]),
 }
@@ -145,7 +152,13 @@ def dtype_code(dt: torch.dtype) -> int:
         raise TypeError(f"trnblas_b200 kernels take float32/bfloat16/float16, got {dt}") from None
 
 
+# the current stream's handle without a Stream object around it (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

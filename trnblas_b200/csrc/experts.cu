@@ -61,22 +61,36 @@ int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups,
   const int64_t sa = round_up(lda * rows, 8);
   // Row tiles of 64 where a group has at most 48 rows on average: eight
   // pipeline stages instead of four keep more weight bytes in flight, which is
-  // what bounds a few rows a group.
+  // what bounds a few rows a group. Longer groups go to CTA pairs when there
+  // are weight columns for both.
   const bool small = rows <= 48 * groups;
-  CUtensorMap mw, mx, mx64;
-  const bool ok = (transB ? encode_map_3d(&mw, dt, 2, B, K, N, nb, ldb, sb, 64, 128)
-                          : encode_map_3d(&mw, dt, 2, B, N, K, nb, ldb, sb, 64, 64)) &&
-                  encode_map_3d(&mx, dt, 2, A, K, rows, 1, lda, sa, 64, small ? 64 : 256) &&
-                  encode_map_3d(&mx64, dt, 2, A, K, rows, 1, lda, sa, 64, 64);
+  const bool pair = !small && N > 128;
+  const bool wide = pair && !transB && N % 64 == 0;  // both 64-column blocks in one copy
+  CUtensorMap mw, mx, mxs;
+  bool ok;
+  if (transB) {
+    ok = encode_map_3d(&mw, dt, 2, B, K, N, nb, ldb, sb, 64, 128);
+  } else if (wide) {
+    const uint64_t dims[4] = {64, static_cast<uint64_t>(K), static_cast<uint64_t>(N / 64), static_cast<uint64_t>(nb)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(ldb), 64, static_cast<uint64_t>(sb)};
+    const uint32_t box[4] = {64, 64, 2, 1};
+    ok = encode_map(&mw, dt, 2, B, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  } else {
+    ok = encode_map_3d(&mw, dt, 2, B, N, K, nb, ldb, sb, 64, 64);
+  }
+  ok = ok && encode_map_3d(&mx, dt, 2, A, K, rows, 1, lda, sa, 64, pair ? 128 : small ? 64 : 256) &&
+       encode_map_3d(&mxs, dt, 2, A, K, rows, 1, lda, sa, 64, pair ? 32 : 64);
   if (!ok) return TRNBLAS_ERR_ALIGN;
   ExpertsParams p{};
   if (int rc = fill_experts(p, out_dtype, rows, groups, N, K, alpha, group_sizes, sizes_64, beta, C, ldc, D, ldd))
     return rc;
   p.in_fmt = dtype == TRNBLAS_BF16 ? kFmtBF16 : kFmtF16;
-  p.w_mn = transB ? 0 : 1;
+  p.w_mn = transB ? 0 : wide ? 2 : 1;
   p.w_shared = shared;
-  return small ? launch_experts<kExpF16, 64>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream))
-               : launch_experts<kExpF16, 256>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (small) return launch_experts<kExpF16, 64>(mw, mx, mxs, mw, mw, p, st);
+  if (pair) return launch_experts_pair<kExpF16, 256>(mw, mx, mxs, mw, mw, p, st);
+  return launch_experts<kExpF16, 256>(mw, mx, mxs, mw, mw, p, st);
 }
 
 int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t M, int64_t N,

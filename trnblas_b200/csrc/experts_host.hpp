@@ -5,7 +5,7 @@
 #include <algorithm>
 #include <string>
 
-#include "experts_sm100.cuh"
+#include "experts_pair_sm100.cuh"
 #include "runtime.hpp"
 
 namespace tb {
@@ -38,6 +38,40 @@ inline int smem_attribute(const void* kernel, int bytes, bool (&done)[64]) {
   return TRNBLAS_OK;
 }
 
+inline cudaLaunchConfig_t pair_config(cudaLaunchAttribute (&attr)[1], int threads, int smem,
+                                      cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (num_sms() / 2)), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// CTA pairs that fit on the device at once, asked once per kernel and device.
+template <typename Kernel>
+int resident_pairs(Kernel kern, const cudaLaunchConfig_t& cfg, int (&cache)[64], int& pairs) {
+  const int dev = current_device();
+  if (dev >= 0 && dev < 64 && cache[dev]) {
+    pairs = cache[dev];
+    return TRNBLAS_OK;
+  }
+  cudaError_t e = cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+  if (pairs < 1) {
+    set_error("no CTA pair fits on this device");
+    return TRNBLAS_ERR_CUDA;
+  }
+  if (dev >= 0 && dev < 64) cache[dev] = pairs;
+  return TRNBLAS_OK;
+}
+
 inline int fill_experts(ExpertsParams& p, int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K,
                         float alpha, const void* sizes, int sizes_64, float beta, const void* C, int64_t ldc,
                         void* D, int64_t ldd) {
@@ -54,31 +88,59 @@ inline int fill_experts(ExpertsParams& p, int out_dtype, int64_t rows, int64_t g
   p.ldc = ldc;
   p.D = D;
   p.ldd = ldd;
-  p.tiles_w = static_cast<int>(ceil_div(N, 128));
   p.status = status_word();
   if (!p.status) return TRNBLAS_ERR_CUDA;
   p.timeout_ns = wait_timeout_ns();
   return TRNBLAS_OK;
 }
 
+// Sets p.tiles_w for weight tiles of `wt` columns and gives an upper bound of
+// the tiles (at most one partly filled row tile a group, and the rows behind
+// the last), or 0 with the error set.
+inline long long bound_tiles(ExpertsParams& p, int bn, int wt) {
+  p.tiles_w = static_cast<int>(ceil_div(p.N, wt));
+  const long long tiles =
+      (ceil_div(p.rows, bn) + std::min<long long>(p.groups, p.rows) + 1) * static_cast<long long>(p.tiles_w);
+  if (tiles <= (1ll << 30)) return tiles;
+  set_error("grouped product: too many tiles");
+  return 0;
+}
+
 template <int KIND, int BN>
 int launch_experts(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorMap& mx64,
-                   const ExpertsParams& p, cudaStream_t stream) {
+                   const CUtensorMap& msw, const CUtensorMap& msx, ExpertsParams& p, cudaStream_t stream) {
   using Cfg = ExpCfg<KIND, BN>;
-  // at most one partly filled row tile a group, and the rows behind the last
-  const long long tiles =
-      (ceil_div(p.rows, BN) + std::min<long long>(p.groups, p.rows) + 1) * static_cast<long long>(p.tiles_w);
-  if (tiles > (1ll << 30)) {
-    set_error("grouped product: too many tiles");
-    return TRNBLAS_ERR_ARG;
-  }
+  const long long tiles = bound_tiles(p, BN, 128);
+  if (!tiles) return TRNBLAS_ERR_ARG;
   auto kern = experts_kernel<KIND, BN>;
   static bool attr_set[64] = {};
   if (int rc = smem_attribute(reinterpret_cast<const void*>(kern), Cfg::SMEM, attr_set)) return rc;
   const int grid = static_cast<int>(std::min<long long>(tiles, num_sms()));
-  kern<<<grid, Cfg::THREADS, Cfg::SMEM, stream>>>(mw, mx, mx64, p);
+  kern<<<grid, Cfg::THREADS, Cfg::SMEM, stream>>>(mw, mx, mx64, msw, msx, p);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "grouped product kernel launch");
+}
+
+// Clusters of two CTAs, as many as can be resident at once (a cluster's CTAs
+// wait for one another only).
+template <int KIND, int BN>
+int launch_experts_pair(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorMap& mx32,
+                        const CUtensorMap& msw, const CUtensorMap& msx, ExpertsParams& p,
+                        cudaStream_t stream) {
+  using Cfg = ExpPairCfg<KIND, BN>;
+  const long long tiles = bound_tiles(p, BN, 256);
+  if (!tiles) return TRNBLAS_ERR_ARG;
+  auto kern = experts_pair_kernel<KIND, BN>;
+  static bool attr_set[64] = {};
+  static int max_pairs[64] = {};
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = pair_config(attr, Cfg::THREADS, Cfg::SMEM, stream);
+  if (int rc = smem_attribute(reinterpret_cast<const void*>(kern), Cfg::SMEM, attr_set)) return rc;
+  int pairs = 0;
+  if (int rc = resident_pairs(kern, cfg, max_pairs, pairs)) return rc;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<long long>(tiles, pairs)), 1, 1);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, mx, mx32, msw, msx, static_cast<const ExpertsParams>(p));
+  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "grouped product pair kernel launch");
 }
 
 }  // namespace tb

@@ -22,11 +22,17 @@
 //   kExpF16  bf16 / fp16, fp32 accumulate; weights stored N x K (K-major) or
 //            K x N (MN-major), no transposed copy;
 //   kExpMx4  E2M1 pairs with one power of two per 32 values along K
-//            (kind::mxf4, block scaled by the tensor core): two scale warps
-//            bring the scale words by 4-byte cp.async straight into the
-//            32 x 16-byte order that tcgen05.cp copies to TMEM, so rows may
-//            start anywhere. Each pipeline stage has its own TMEM scale
-//            columns, which its empty barrier frees with the stage.
+//            (kind::mxf4, block scaled by the tensor core). The scales lie in
+//            blocks of 128 rows x 128 K (512 bytes) in the order that tcgen05.cp
+//            copies to TMEM, the word of a row's four blocks at 16 * (row % 32)
+//            + 4 * (row / 32 % 4), so TMA brings them with the operands. Groups
+//            start at any row, but their scales at a block of their own; a
+//            tile starts at a multiple of 64 rows of its group. Each pipeline
+//            stage has its own TMEM scale columns, which its empty barrier frees
+//            with the stage. (Scale words in row order, brought and reordered
+//            by warps of the kernel, cost 1.7 times the time at 8192^3 on CTA
+//            pairs: their loads, proxy fences and arrivals were the slowest
+//            part of every stage.)
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -35,10 +41,12 @@ namespace tb {
 
 enum ExpKind : int { kExpF16 = 0, kExpMx4 = 1 };
 constexpr int kMaxGroups = 1024;
+constexpr int kGroupTableBytes = (kMaxGroups + 2) * 12;
 
 struct GroupTable {
   int* row0;   // [G + 2] first row of each group; [G] the rows behind the last group, [G + 1] rows
   int* tile0;  // [G + 2] first tile; [G + 1] all tiles
+  int* blk0;   // [G + 1] first scale block (of 128 rows), kExpMx4
 };
 
 struct ExpertsParams {
@@ -56,11 +64,7 @@ struct ExpertsParams {
   void* D;
   long long ldd;
   int tiles_w;  // weight tiles of 128
-  // kExpMx4: scale words [K / 128][rows] of the rows and of the weights
-  const uint32_t* xs;
-  long long xs_rows;
-  const uint32_t* ws;
-  long long ws_rows;
+  int w_blocks;  // kExpMx4: scale blocks of one weight matrix
   int* status;
   unsigned long long timeout_ns;
 };
@@ -70,13 +74,14 @@ __device__ __forceinline__ long long load_size(const void* sizes, int sizes64, i
                  : static_cast<long long>(__ldg(reinterpret_cast<const int*>(sizes) + g));
 }
 
-// One warp: the first row of every group, and the first tile with `bn` rows to
-// a tile at most and `per` tiles for each of them (bn 0: rows only).
+// One warp: the first row of every group, the first tile with `bn` rows to a
+// tile at most and `per` tiles for each of them (bn 0: none), and the first
+// scale block (tb.blk0 null: none).
 __device__ __forceinline__ void build_groups(const GroupTable& tb, const void* sizes, int sizes64,
                                              int groups, int rows, int bn, int per, int* status) {
   const int lane = threadIdx.x & 31;
   long long run = 0;
-  int tiles = 0;
+  int tiles = 0, blocks = 0;
   bool bad = false;
   for (int base = 0; base < groups; base += 32) {
     const int g = base + lane;
@@ -104,6 +109,17 @@ __device__ __forceinline__ void build_groups(const GroupTable& tb, const void* s
       tb.row0[g] = lo;
       if (bn) tb.tile0[g] = tiles + tinc - nt;
     }
+    if (tb.blk0) {
+      const int nb = (hi - lo + 127) >> 7;
+      int binc = nb;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, binc, o);
+        if (lane >= o) binc += u;
+      }
+      if (g < groups) tb.blk0[g] = blocks + binc - nb;
+      blocks += __shfl_sync(0xffffffffu, binc, 31);
+    }
     run += __shfl_sync(0xffffffffu, inc, 31);
     tiles += __shfl_sync(0xffffffffu, tinc, 31);
   }
@@ -114,6 +130,7 @@ __device__ __forceinline__ void build_groups(const GroupTable& tb, const void* s
     const int end = static_cast<int>(run < rows ? run : rows);
     tb.row0[groups] = end;
     tb.row0[groups + 1] = rows;
+    if (tb.blk0) tb.blk0[groups] = blocks;
     if (bn) {
       tb.tile0[groups] = tiles;
       tb.tile0[groups + 1] = tiles + ((rows - end + bn - 1) / bn) * per;
@@ -125,11 +142,13 @@ struct ExpTile {
   int g;       // group, or `groups` for the rows behind the last one
   int r0, nv;  // first row and number of rows
   int n0;      // first weight column
+  int x0;      // first row within the group
 };
 
 // Tile t: the tiles of one weight block are next to one another, so the CTAs
-// that run together share it and the group's rows.
-template <int BN>
+// that run together share it and the group's rows. BN: most rows of a tile, a
+// multiple of STEP; WT: weight columns of a tile.
+template <int BN, int STEP = 16, int WT = 128>
 __device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, int t) {
   int lo = 0, hi = groups + 1;  // tile0[lo] <= t < tile0[hi]
   while (hi - lo > 1) {
@@ -141,14 +160,15 @@ __device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, in
   e.g = lo;
   const int first = tb.row0[lo], m = tb.row0[lo + 1] - first;
   const int nt = (m + BN - 1) / BN;
-  // equal tiles, a multiple of 16 rows each (the last one keeps the rest;
+  // equal tiles, a multiple of STEP rows each (the last one keeps the rest;
   // never empty, since nt - 1 tiles of at most BN rows do not cover m)
-  const int step = ((m + nt - 1) / nt + 15) & ~15;
+  const int step = ((m + nt - 1) / nt + STEP - 1) & ~(STEP - 1);
   const int i = t - tb.tile0[lo];
   const int w = i / nt, x = i - w * nt;
-  e.r0 = first + x * step;
+  e.x0 = x * step;
+  e.r0 = first + e.x0;
   e.nv = min(step, m - x * step);
-  e.n0 = w * 128;
+  e.n0 = w * WT;
   return e;
 }
 
@@ -158,21 +178,24 @@ struct ExpCfg {
   static constexpr int BK = MX ? 256 : 64;  // one 128-byte swizzle row of K
   static constexpr int W_TILE = 128 * 128;
   static constexpr int X_TILE = BN * 128;
-  static constexpr int XBLK = (BN + 127) / 128;       // 128-row scale blocks of the rows
-  static constexpr int SFW = MX ? 2 * 512 : 0;        // two scale words (K = 128 each)
+  // rows start at a multiple of STEP in their group; with 64 a tile of 64 rows
+  // lies in one scale block and one of 192 in two
+  static constexpr int STEP = MX ? 64 : 16;
+  static constexpr int XBLK = (BN + 127) / 128;       // scale blocks of the rows
+  static_assert(!MX || BN == 64 || BN == 192, "scale blocks of a tile");
+  static constexpr int SFW = MX ? 2 * 512 : 0;        // K = 256 is two blocks
   static constexpr int SFX = MX ? 2 * XBLK * 512 : 0;
   static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle atom's alignment");
   // what fits beside 16 KB of epilogue blocks and the group table; at most 8
-  static constexpr int FIT = (227 * 1024 - 1024 - 512 - kEpiStageBytes - (kMaxGroups + 2) * 8) / STAGE_BYTES;
+  static constexpr int FIT = (227 * 1024 - 1024 - 512 - kEpiStageBytes - kGroupTableBytes) / STAGE_BYTES;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SF_COLS = MX ? 2 * 4 * (1 + XBLK) : 0;  // TMEM scale columns of a stage
   static constexpr int COLS = 2 * BN + STAGES * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static_assert(COLS <= 512, "accumulators and scales fit TMEM");
-  static constexpr int SCALE_WARPS = MX ? 2 : 0;
-  static constexpr int THREADS = 32 * (6 + SCALE_WARPS);
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + kEpiStageBytes + (kMaxGroups + 2) * 8;
+  static constexpr int THREADS = 32 * 6;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + kEpiStageBytes + kGroupTableBytes;
 };
 
 // Instruction descriptor of kind::mxf4 with E8M0 scales: E2M1 operands, N / 8
@@ -199,17 +222,6 @@ __device__ __forceinline__ void mma_mx4(uint32_t d_tmem, uint64_t adesc, uint64_
 // r % 32, column r / 32.
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-
-// 4 bytes global -> shared, zero when !ok (src is not read then).
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
-  const uint32_t n = ok ? 4u : 0u;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Forward epilogue of one warp's block: lane l holds v[j] = accumulator of
@@ -275,11 +287,15 @@ __device__ __forceinline__ void exp_store(const ExpertsParams& p, int r0, int le
 // map_w: the weights (kExpF16: K-major boxes of 64 K x 128 N, or MN-major of
 // 64 N x 64 K; kExpMx4: 128 bytes x 128 rows). map_x / map_x64: the rows, in
 // boxes of BN and of 64 rows (a tile of few rows loads only what it needs).
+// map_sw / map_sx (kExpMx4): the scales as 128 words x K blocks x row blocks,
+// in boxes of 2 K blocks and 1 / XBLK row blocks.
 template <int KIND, int BN>
 __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     experts_kernel(const __grid_constant__ CUtensorMap map_w,
                    const __grid_constant__ CUtensorMap map_x,
-                   const __grid_constant__ CUtensorMap map_x64, const ExpertsParams p) {
+                   const __grid_constant__ CUtensorMap map_x64,
+                   const __grid_constant__ CUtensorMap map_sw,
+                   const __grid_constant__ CUtensorMap map_sx, const ExpertsParams p) {
   using Cfg = ExpCfg<KIND, BN>;
   constexpr int STAGES = Cfg::STAGES;
   constexpr uint32_t SB = Cfg::STAGE_BYTES;
@@ -298,14 +314,15 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   GroupTable tb;
   tb.row0 = reinterpret_cast<int*>(epi + kEpiStageBytes);
   tb.tile0 = tb.row0 + kMaxGroups + 2;
+  tb.blk0 = Cfg::MX ? tb.tile0 + kMaxGroups + 2 : nullptr;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
   const Abort ab{abort_flag, p.status, p.timeout_ns};
 
   if (threadIdx.x == 32) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1 + Cfg::SCALE_WARPS);
+      mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -318,6 +335,10 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
     tma_prefetch_desc(&map_x64);
+    if (Cfg::MX) {
+      tma_prefetch_desc(&map_sw);
+      tma_prefetch_desc(&map_sx);
+    }
   }
   if (warp == 0)
     build_groups(tb, p.sizes, p.sizes64, p.groups, p.rows, BN, p.tiles_w, p.status);
@@ -326,27 +347,27 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
   const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
   const int num_tiles = tb.tile0[p.groups + 1];
   // tiles with products; the ones behind are stores of beta * C alone
   const int work_tiles = num_kb ? tb.tile0[p.groups] : 0;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
+    if (elect_one()) {
     // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0;
-    bool aborted = false;
-    for (int t = blockIdx.x; t < work_tiles && !aborted; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+    const bool aborted = [&] {
+    for (int t = blockIdx.x; t < work_tiles; t += gridDim.x) {
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
       // above three quarters of the tile one full box, else boxes of 64 rows
       const int boxes = (BN == 64 || e.nv > BN * 3 / 4) ? 0 : (e.nv + 63) / 64;
-      const uint32_t bytes = Cfg::W_TILE + (boxes ? boxes * 64 * 128 : Cfg::X_TILE);
+      const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * 64 * 128 : Cfg::X_TILE);
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
-          aborted = true;
-          break;
+          return true;
         }
         uint8_t* sw = smem + stage * SB;
         uint8_t* sx = sw + Cfg::W_TILE;
@@ -357,6 +378,9 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
           if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
           for (int j = 0; j < boxes; ++j)
             tma_load_3d(sx + j * 8192, &map_x64, &full_bar[stage], k0, e.r0 + 64 * j, 0);
+          uint8_t* sf = sx + Cfg::X_TILE;
+          tma_load_3d(sf, &map_sw, &full_bar[stage], 0, 2 * kb, e.g * p.w_blocks + (e.n0 >> 7));
+          tma_load_3d(sf + Cfg::SFW, &map_sx, &full_bar[stage], 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
         } else {
           const int k0 = kb * Cfg::BK;
           const int gw = p.w_shared ? 0 : e.g;
@@ -376,14 +400,22 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
         }
       }
     }
+      return false;
+    }();
     if (aborted || ab.raised()) {
       // let copies already issued land before the CTA exits (bounded)
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 20000000ull) {
       }
     }
-  } else if (warp == 1 && lane == 0) {
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
+    // The whole warp walks the tiles, one elected lane issues a tile's K loop:
+    // one loop with warp-uniform bounds inside the election keeps descriptors
+    // and addresses in uniform registers (nested loops there did not: 130
+    // cycles an instruction on CTA pairs).
     const uint32_t sw0 = smem_u32(smem), sx0 = sw0 + Cfg::W_TILE;
     uint64_t wd[4], xd[4];
 #pragma unroll
@@ -395,60 +427,72 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     const uint64_t sfd = sdesc_kmajor_noswz(sx0 + Cfg::X_TILE, 128, 128);
     int stage = 0, tc = 0;
     uint32_t phase = 0;
-    bool stop = false;
-    for (int t = blockIdx.x; t < work_tiles && !stop; t += gridDim.x, ++tc) {
-      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
-      const uint32_t nm = static_cast<uint32_t>((e.nv + 15) & ~15);
+    for (int t = blockIdx.x; t < work_tiles; t += gridDim.x, ++tc) {
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
+      const uint32_t nm = warp_uniform(static_cast<uint32_t>((e.nv + 15) & ~15));
+      const uint32_t xcol = warp_uniform(static_cast<uint32_t>(e.x0 >> 5) & 3u);  // in its scale block
       const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn, 0, 128, nm);
       const uint32_t id2 = idesc_mx4(nm, 2);
       const int buf = tc & 1;
-      if (!mbar_wait(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
+      if (!mbar_wait_warp(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
       tc_fence_after();
       const uint32_t d = tmem_base + buf * BN;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&full_bar[stage], phase, ab, kTimeoutFull)) {
-          stop = true;
+      bool ok = true;
+      if (elect_one()) {
+        int s = stage;
+        uint32_t ph = phase;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full_bar[s], ph, ab, kTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t off = s * SB;
+          if constexpr (Cfg::MX) {
+            const uint32_t sfw = tmem_base + 2 * BN + s * Cfg::SF_COLS;
+            const uint32_t sfx = sfw + 8;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              tmem_cp_scales(sfw + 4 * w, sdesc_add(sfd, off + w * 512));
+#pragma unroll
+              for (int b = 0; b < Cfg::XBLK; ++b)
+                tmem_cp_scales(sfx + 4 * (w * Cfg::XBLK + b),
+                               sdesc_add(sfd, off + Cfg::SFW + (b * 2 + w) * 512));
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_mx4(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), (kk & 1) ? id2 : id,
+                      sfw + 4 * (kk >> 1), sfx + 4 * Cfg::XBLK * (kk >> 1) + xcol, (kb | kk) ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f16(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), id, (kb | kk) ? 1u : 0u);
+          }
+          tc_commit(&empty_bar[s]);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) tc_commit(&accf_bar[buf]);
+      }
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int adv = stage + num_kb;
+      stage = adv % STAGES;
+      phase ^= static_cast<uint32_t>(adv / STAGES) & 1u;
+    }
+    // Every MMA this warp issued must finish before TMEM is released.
+    if (elect_one()) {
+      tc_commit(drain_bar);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain_bar, 0)) {
+        if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
+          ab.raise(kTimeoutDrain);
           break;
         }
-        tc_fence_after();
-        const uint32_t off = stage * SB;
-        if constexpr (Cfg::MX) {
-          const uint32_t sfw = tmem_base + 2 * BN + stage * Cfg::SF_COLS;
-          const uint32_t sfx = sfw + 8;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            tmem_cp_scales(sfw + 4 * w, sdesc_add(sfd, off + w * 512));
-#pragma unroll
-            for (int b = 0; b < Cfg::XBLK; ++b)
-              tmem_cp_scales(sfx + 4 * (w * Cfg::XBLK + b),
-                             sdesc_add(sfd, off + Cfg::SFW + (w * Cfg::XBLK + b) * 512));
-          }
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_mx4(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), (kk & 1) ? id2 : id,
-                    sfw + 4 * (kk >> 1), sfx + 4 * Cfg::XBLK * (kk >> 1), (kb | kk) ? 1u : 0u);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f16(d, sdesc_add(wd[kk], off), sdesc_add(xd[kk], off), id, (kb | kk) ? 1u : 0u);
-        }
-        tc_commit(&empty_bar[stage]);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!stop) tc_commit(&accf_bar[buf]);
-    }
-    // Every MMA this thread issued must finish before TMEM is released.
-    tc_commit(drain_bar);
-    const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(drain_bar, 0)) {
-      if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
-        ab.raise(kTimeoutDrain);
-        break;
       }
     }
+    __syncwarp();
   } else if (warp >= 2 && warp < 6) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;  // TMEM lane quarter
@@ -456,7 +500,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     int tc = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
       const int n0 = e.n0 + 32 * q;
       if (t >= work_tiles) {
         float z[32];
@@ -486,61 +530,6 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&acce_bar[buf]);
     }
-  } else if (Cfg::MX && warp >= 6) {
-    // ------------------------------------------------------------ scales
-    // Warp 6 + w brings scale word w of every stage (K = 128), two stages in
-    // flight behind the one being asked for.
-    const int w = warp - 6;
-    const int kwords = (p.K + 127) / 128;
-    const uint32_t s0 = smem_u32(smem) + Cfg::W_TILE + Cfg::X_TILE;
-    int stage = 0, sig = 0, pending = 0;
-    uint32_t phase = 0;
-    bool stop = false;
-    auto signal = [&] {
-      fence_proxy_async_smem();  // tcgen05.cp reads what the copies wrote
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full_bar[sig]);
-      if (++sig == STAGES) sig = 0;
-      --pending;
-    };
-    for (int t = blockIdx.x; t < work_tiles && !stop; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN>(tb, p.groups, t);
-      const uint32_t* wrow = p.ws + static_cast<long long>(e.g) * p.N + e.n0;
-      const uint32_t* xrow = p.xs + e.r0;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1u, ab, kTimeoutAux)) {
-          stop = true;
-          break;
-        }
-        const int kw = kb * 2 + w;
-        const bool kok = kw < kwords;
-        const uint32_t dst = s0 + stage * SB + lane * 16;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int i = lane + 32 * c;
-          const bool ok = kok && e.n0 + i < p.N;
-          cp_async4(dst + w * 512 + 4 * c, ok ? wrow + static_cast<long long>(kw) * p.ws_rows + i : p.ws, ok);
-        }
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          const int i = lane + 32 * c;
-          const bool ok = kok && i < e.nv;
-          cp_async4(dst + Cfg::SFW + w * Cfg::XBLK * 512 + (c >> 2) * 512 + (c & 3) * 4,
-                    ok ? xrow + static_cast<long long>(kw) * p.xs_rows + i : p.xs, ok);
-        }
-        cp_async_commit();
-        if (++pending > 2) {
-          cp_async_wait<2>();
-          signal();
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    cp_async_wait<0>();
-    while (pending) signal();
   }
 
   tc_fence_before();

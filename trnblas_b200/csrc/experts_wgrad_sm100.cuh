@@ -53,9 +53,9 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   GroupTable tb;
   tb.row0 = reinterpret_cast<int*>(smem + STAGES * SB + 512);
-  tb.tile0 = nullptr;
+  tb.tile0 = tb.blk0 = nullptr;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
   const Abort ab{abort_flag, p.status, p.timeout_ns};
 
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
   const int per_group = p.tiles_m * p.tiles_n;
   struct Tile {
@@ -98,17 +98,17 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
     return e;
   };
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
+    if (elect_one()) {
     // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0;
-    bool aborted = false;
-    for (int t = blockIdx.x; t < p.num_tiles && !aborted; t += gridDim.x) {
+    const bool aborted = [&] {
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
       const Tile e = tile(t);
       for (int r = 0; r < e.m; r += Cfg::BK) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
-          aborted = true;
-          break;
+          return true;
         }
         uint8_t* sa = smem + stage * SB;
         uint8_t* sb = sa + Cfg::A_TILE;
@@ -125,13 +125,21 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
         }
       }
     }
+      return false;
+    }();
     if (aborted || ab.raised()) {
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 20000000ull) {
       }
     }
-  } else if (warp == 1 && lane == 0) {
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
+    // The whole warp walks the tiles, one elected lane issues a tile's K loop:
+    // one loop with warp-uniform bounds inside the election keeps descriptors
+    // and addresses in uniform registers (nested loops there did not: 130
+    // cycles an instruction on CTA pairs).
     const uint32_t id = idesc(kAccF32, w.in_fmt, w.in_fmt, 1, 1, Cfg::BM, Cfg::BN);
     const uint32_t sa0 = smem_u32(smem), sb0 = sa0 + Cfg::A_TILE;
     uint64_t ad[4], bd[4];
@@ -142,43 +150,56 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
     }
     int stage = 0, tc = 0;
     uint32_t phase = 0;
-    bool stop = false;
-    for (int t = blockIdx.x; t < p.num_tiles && !stop; t += gridDim.x) {
-      const Tile e = tile(t);
-      if (e.m == 0) continue;
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
+      const int m = warp_uniform(tile(t).m);
+      if (m == 0) continue;
       const int buf = tc & 1;
-      if (!mbar_wait(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
+      if (!mbar_wait_warp(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
       ++tc;
       tc_fence_after();
       const uint32_t d = tmem_base + buf * Cfg::BN;
-      for (int r = 0; r < e.m; r += Cfg::BK) {
-        if (!mbar_wait(&fix_bar[stage], phase, ab, kTimeoutFull)) {
-          stop = true;
+      const int blocks = (m + Cfg::BK - 1) / Cfg::BK;
+      bool ok = true;
+      if (elect_one()) {
+        int s = stage;
+        uint32_t ph = phase;
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(&fix_bar[s], ph, ab, kTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t off = s * SB;
+          const int steps = (m - kb * Cfg::BK + 15) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < steps)
+              mma_f16(d, sdesc_add(ad[kk], off), sdesc_add(bd[kk], off), id, (kb | kk) ? 1u : 0u);
+          tc_commit(&empty_bar[s]);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) tc_commit(&accf_bar[buf]);
+      }
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int adv = stage + blocks;
+      stage = adv % STAGES;
+      phase ^= static_cast<uint32_t>(adv / STAGES) & 1u;
+    }
+    // Every MMA this warp issued must finish before TMEM is released.
+    if (elect_one()) {
+      tc_commit(drain_bar);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain_bar, 0)) {
+        if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
+          ab.raise(kTimeoutDrain);
           break;
         }
-        tc_fence_after();
-        const uint32_t off = stage * SB;
-        const int steps = min(4, (e.m - r + 15) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          if (kk < steps)
-            mma_f16(d, sdesc_add(ad[kk], off), sdesc_add(bd[kk], off), id, (r | kk) ? 1u : 0u);
-        tc_commit(&empty_bar[stage]);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!stop) tc_commit(&accf_bar[buf]);
-    }
-    tc_commit(drain_bar);
-    const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(drain_bar, 0)) {
-      if (globaltimer_ns() - t0 > 100000000ull) {  // 100 ms
-        ab.raise(kTimeoutDrain);
-        break;
       }
     }
+    __syncwarp();
   } else if (warp == 6) {
     // ------------------------------------------------------------ fixer
     int stage = 0;

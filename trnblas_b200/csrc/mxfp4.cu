@@ -5,9 +5,10 @@
 // A quantised operand of `rows` x K:
 //   data    rows x ldq bytes, two values a byte (the even one in the low half),
 //           K padded to a multiple of 32 with zeros, ldq a multiple of 16;
-//   scales  [ceil(K / 128)][rows] words of four E8M0 bytes (zero past K): one
-//           word is what a row needs for K = 128, and words of neighbouring
-//           rows are neighbours, so a tile may start at any row.
+//   scales  blocks of 128 rows x 128 K, [row block][ceil(K / 128)][512 bytes]:
+//           the word of a row's four E8M0 bytes (zero past K) at 16 * (r % 32)
+//           + 4 * (r / 32 % 4), as the tensor core's copy wants them. Every
+//           matrix of a stack starts a block of its own.
 #include <cuda_fp4.h>
 
 #include <algorithm>
@@ -80,46 +81,116 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& s) 
   return w;
 }
 
-// A warp takes 4 rows x 256 values, its lanes 8 neighbouring values of a row
-// each: 16-byte loads and 128-byte stores, four of them in flight. Eight warps
-// of a block take 32 neighbouring rows, so the scale words of a K block leave
-// as 128 contiguous bytes. Bounded by the read of X.
-template <typename T>
+// Which rows a scale block holds: local rows 0 .. limit - 1 at `base` + local.
+struct BlockRows {
+  long long base;
+  int local0, limit;
+};
+
+__device__ __forceinline__ BlockRows stack_block(int blk, int rows, int per_matrix) {
+  const int m = blk / per_matrix;
+  return {static_cast<long long>(m) * rows, (blk - m * per_matrix) * 128, rows};
+}
+
+// Groups' blocks (group table in shared memory); limit 0 behind the last one.
+__device__ __forceinline__ BlockRows group_block(const GroupTable& tb, int groups, int blk) {
+  if (blk >= tb.blk0[groups]) return {0, 0, 0};
+  int lo = 0, hi = groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tb.blk0[mid] <= blk) lo = mid;
+    else hi = mid;
+  }
+  return {tb.row0[lo], (blk - tb.blk0[lo]) * 128, tb.row0[lo + 1] - tb.row0[lo]};
+}
+
+struct GroupArgs {
+  const void* sizes;  // nullptr: a stack of matrices of `rows` rows
+  int sizes64, groups, rows;
+  int* status;
+};
+
+// The group table of a quantising or regrouping block (all threads).
+__device__ __forceinline__ GroupTable block_table(int* mem, const GroupArgs& ga) {
+  GroupTable tb{mem, nullptr, mem + kMaxGroups + 2};
+  if (threadIdx.x < 32) build_groups(tb, ga.sizes, ga.sizes64, ga.groups, ga.rows, 0, 0, ga.status);
+  __syncthreads();
+  return tb;
+}
+
+// A warp takes 4 rows 32 apart x 256 values, its lanes 8 neighbouring values of
+// a row each: 16-byte loads, four in flight, and 128-byte stores. The four
+// rows' scale words are neighbours, and the eight warps of a block hold
+// neighbouring ones, so a K block's words leave as 128 contiguous bytes.
+// Blocks walk K with stride gridDim.y. Bounded by the read of X.
+template <typename T, bool GROUPED>
 __global__ void __launch_bounds__(256)
-    mxfp4_quantize_kernel(const T* __restrict__ X, long long ldx, int rows, int K, int vec,
-                          uint8_t* __restrict__ data, long long ldq, uint32_t* __restrict__ scales) {
+    mxfp4_quantize_kernel(const T* __restrict__ X, long long ldx, GroupArgs ga, int per_matrix, int K, int vec,
+                          uint8_t* __restrict__ data, long long ldq, uint4* __restrict__ scales) {
+  __shared__ int mem[GROUPED ? 2 * (kMaxGroups + 2) : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r0 = blockIdx.x * 32 + warp * 4;
-  const int k = blockIdx.y * 256 + lane * 8;
+  const int blk = blockIdx.x >> 2;
+  BlockRows br;
+  if constexpr (GROUPED) {
+    const GroupTable tb = block_table(mem, ga);
+    br = group_block(tb, ga.groups, blk);
+    if (br.limit == 0) return;
+  } else {
+    br = stack_block(blk, ga.rows, per_matrix);
+  }
+  const int l32 = (blockIdx.x & 3) * 8 + warp;  // row % 32
+  const int l0 = br.local0 + l32;
   const int kwords = (K + 127) >> 7;
-  float x[4][8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    load8(X + (r0 + i < rows ? static_cast<long long>(r0 + i) * ldx + k : 0), r0 + i < rows ? K - k : 0, vec, x[i]);
-  uint32_t word[4];
+  bool ok[4];
+  long long row[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t s;
-    const uint32_t w = quantize8(x[i], s);
-    if (r0 + i < rows && (k >> 1) < ldq)
-      *reinterpret_cast<uint32_t*>(data + static_cast<long long>(r0 + i) * ldq + (k >> 1)) = w;
-    // the four scale bytes of 16 lanes; past K's last block zero
-    if ((k & ~31) >= K) s = 0;
-    uint32_t b = s << (8 * ((lane >> 2) & 3));
-    b |= __shfl_xor_sync(0xffffffffu, b, 4);
-    b |= __shfl_xor_sync(0xffffffffu, b, 8);
-    word[i] = b;
+    ok[i] = l0 + 32 * i < br.limit;
+    row[i] = ok[i] ? br.base + l0 + 32 * i : br.base;
   }
-  const int kw = k >> 7;
-  if ((lane & 15) == 0 && kw < kwords) {
-    uint32_t* dst = scales + static_cast<long long>(kw) * rows + r0;
-    if (r0 + 4 <= rows && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
-    } else {
+  for (int k = blockIdx.y * 256 + lane * 8; k - lane * 8 < K; k += gridDim.y * 256) {
+    float x[4][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r0 + i < rows) dst[i] = word[i];
+    for (int i = 0; i < 4; ++i) load8(X + row[i] * ldx + (k < K ? k : 0), ok[i] ? K - k : 0, vec, x[i]);
+    uint32_t word[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t s;
+      const uint32_t w = quantize8(x[i], s);
+      if (ok[i] && (k >> 1) < ldq) *reinterpret_cast<uint32_t*>(data + row[i] * ldq + (k >> 1)) = w;
+      // the four scale bytes of 16 lanes; zero past K's last block
+      if ((k & ~31) >= K || !ok[i]) s = 0;
+      uint32_t b = s << (8 * ((lane >> 2) & 3));
+      b |= __shfl_xor_sync(0xffffffffu, b, 4);
+      b |= __shfl_xor_sync(0xffffffffu, b, 8);
+      word[i] = b;
     }
+    const int kw = k >> 7;
+    if ((lane & 15) == 0 && kw < kwords)
+      scales[(static_cast<long long>(blk) * kwords + kw) * 32 + l32] =
+          make_uint4(word[0], word[1], word[2], word[3]);
+  }
+}
+
+// The scales of rows held as one matrix, in blocks that start with the groups.
+// One thread per 16 bytes of the result.
+__global__ void __launch_bounds__(256)
+    mxfp4_regroup_kernel(const uint32_t* __restrict__ src, GroupArgs ga, int kwords, uint4* __restrict__ dst) {
+  __shared__ int mem[2 * (kMaxGroups + 2)];
+  const GroupTable tb = block_table(mem, ga);
+  const int blk = blockIdx.x;
+  const BlockRows br = group_block(tb, ga.groups, blk);
+  if (br.limit == 0) return;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < kwords * 32; i += gridDim.y * 256) {
+    const int kw = i >> 5, l32 = i & 31;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int l = br.local0 + l32 + 32 * j;
+      const long long r = br.base + l;
+      w[j] = l < br.limit ? __ldg(src + ((r >> 7) * kwords + kw) * 128 + (r & 31) * 4 + ((r >> 5) & 3)) : 0u;
+    }
+    dst[(static_cast<long long>(blk) * kwords + kw) * 32 + l32] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -140,44 +211,53 @@ __device__ __forceinline__ __half to_out<__half>(float v) { return __float2half_
 template <typename T>
 __global__ void __launch_bounds__(256)
     mxfp4_dequantize_kernel(const uint8_t* __restrict__ data, long long ldq,
-                            const uint32_t* __restrict__ scales, int rows, int K, int vec,
+                            const uint4* __restrict__ scales, int rows, int per_matrix, int K, int vec,
                             T* __restrict__ Y, long long ldy) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r0 = blockIdx.x * 32 + warp * 4;
-  const int k = blockIdx.y * 256 + lane * 8;
-  if (k >= K) return;
-  uint32_t w[4], sw[4];
+  const int blk = blockIdx.x >> 2;
+  const BlockRows br = stack_block(blk, rows, per_matrix);
+  const int l32 = (blockIdx.x & 3) * 8 + warp;
+  const int l0 = br.local0 + l32;
+  const int kwords = (K + 127) >> 7;
+  if (l0 >= br.limit) return;
+  for (int k = blockIdx.y * 256 + lane * 8; k < K; k += gridDim.y * 256) {
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool ok = r0 + i < rows;
-    w[i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(data + static_cast<long long>(r0 + i) * ldq + (k >> 1))) : 0;
-    sw[i] = ok ? __ldg(scales + static_cast<long long>(k >> 7) * rows + r0 + i) : 0;
-  }
+    for (int i = 0; i < 4; ++i)
+      w[i] = l0 + 32 * i < br.limit
+                 ? __ldg(reinterpret_cast<const uint32_t*>(data + (br.base + l0 + 32 * i) * ldq + (k >> 1)))
+                 : 0;
+    const uint4 s4 = __ldg(scales + (static_cast<long long>(blk) * kwords + (k >> 7)) * 32 + l32);
+    const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (r0 + i >= rows) break;
-    const uint32_t s = (sw[i] >> (8 * ((k >> 5) & 3))) & 0xFFu;
-    const float unit = s == 255 ? __uint_as_float(0x7FC00000u)
-                                : (s == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23));
-    T out[8];
+    for (int i = 0; i < 4; ++i) {
+      if (l0 + 32 * i >= br.limit) break;
+      const uint32_t s = (sw[i] >> (8 * ((k >> 5) & 3))) & 0xFFu;
+      const float unit = s == 255 ? __uint_as_float(0x7FC00000u)
+                                  : (s == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23));
+      T out[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t c = (w[i] >> (4 * j)) & 0xFu;
-      const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(((c & 8u) << 12) | ((c & 7u) << 9))));
-      out[j] = to_out<T>(v * 16384.0f * unit);
-    }
-    T* dst = Y + static_cast<long long>(r0 + i) * ldy + k;
-    if (vec && k + 8 <= K) {
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t c = (w[i] >> (4 * j)) & 0xFu;
+        const float v =
+            __half2float(__ushort_as_half(static_cast<unsigned short>(((c & 8u) << 12) | ((c & 7u) << 9))));
+        out[j] = to_out<T>(v * 16384.0f * unit);
+      }
+      T* dst = Y + (br.base + l0 + 32 * i) * ldy + k;
+      if (vec && k + 8 <= K) {
 #pragma unroll
-      for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
-        reinterpret_cast<uint4*>(dst)[h] = reinterpret_cast<const uint4*>(out)[h];
-    } else {
+        for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
+          reinterpret_cast<uint4*>(dst)[h] = reinterpret_cast<const uint4*>(out)[h];
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k + j < K) dst[j] = out[j];
+        for (int j = 0; j < 8; ++j)
+          if (k + j < K) dst[j] = out[j];
+      }
     }
   }
 }
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_mx(const char* what, int64_t rows, int64_t K, int64_t ldq) {
   const int64_t lim = (1ll << 31) - 512;
@@ -189,86 +269,17 @@ int check_mx(const char* what, int64_t rows, int64_t K, int64_t ldq) {
     set_error(std::string(what) + ": a row of packed values takes round_up(K, 32) / 2 bytes at a stride of a multiple of 16");
     return TRNBLAS_ERR_ARG;
   }
-  if (ceil_div(K, 256) > 65535) {
-    set_error(std::string(what) + ": K above 65535 * 256");
-    return TRNBLAS_ERR_ARG;
-  }
   return TRNBLAS_OK;
 }
 
-bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of a CTA pair's tile: two accumulators of 192 columns and the scales of
+// five stages fill TMEM.
+constexpr int kMxPairBN = 192;
 
-}  // namespace
-}  // namespace tb
 
-using namespace tb;
-
-extern "C" {
-
-int trnblas_mxfp4_quantize(int dtype, int64_t rows, int64_t K, const void* X, int64_t ldx, void* data,
-                           int64_t ldq, void* scales, void* stream_) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (dtype != TRNBLAS_F32 && dtype != TRNBLAS_BF16 && dtype != TRNBLAS_F16) {
-    set_error("trnblas_mxfp4_quantize: dtype must be F32, BF16 or F16");
-    return TRNBLAS_ERR_ARG;
-  }
-  if (int rc = check_mx("trnblas_mxfp4_quantize", rows, K, ldq)) return rc;
-  if (rows == 0 || K == 0) return TRNBLAS_OK;
-  if (!X || !data || !scales || ldx < K || !al16(data) || (reinterpret_cast<uintptr_t>(scales) & 3)) {
-    set_error("trnblas_mxfp4_quantize: NULL or unaligned operand, or ldx smaller than K");
-    return TRNBLAS_ERR_ARG;
-  }
-  const dim3 grid(static_cast<unsigned>(ceil_div(rows, 32)), static_cast<unsigned>(ceil_div(K, 256)));
-  const int es = dtype == TRNBLAS_F32 ? 4 : 2;
-  const int vec = al16(X) && (ldx * es) % 16 == 0;
-  uint8_t* q = static_cast<uint8_t*>(data);
-  uint32_t* s = static_cast<uint32_t*>(scales);
-  const int r = static_cast<int>(rows), k = static_cast<int>(K);
-  if (dtype == TRNBLAS_F32)
-    mxfp4_quantize_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float*>(X), ldx, r, k, vec, q, ldq, s);
-  else if (dtype == TRNBLAS_BF16)
-    mxfp4_quantize_kernel<__nv_bfloat16>
-        <<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(X), ldx, r, k, vec, q, ldq, s);
-  else
-    mxfp4_quantize_kernel<__half><<<grid, 256, 0, stream>>>(static_cast<const __half*>(X), ldx, r, k, vec, q, ldq, s);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "mxfp4 quantise kernel launch");
-}
-
-int trnblas_mxfp4_dequantize(int dtype, int64_t rows, int64_t K, const void* data, int64_t ldq,
-                             const void* scales, void* Y, int64_t ldy, void* stream_) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (dtype != TRNBLAS_F32 && dtype != TRNBLAS_BF16 && dtype != TRNBLAS_F16) {
-    set_error("trnblas_mxfp4_dequantize: dtype must be F32, BF16 or F16");
-    return TRNBLAS_ERR_ARG;
-  }
-  if (int rc = check_mx("trnblas_mxfp4_dequantize", rows, K, ldq)) return rc;
-  if (rows == 0 || K == 0) return TRNBLAS_OK;
-  if (!Y || !data || !scales || ldy < K || !al16(data) || (reinterpret_cast<uintptr_t>(scales) & 3)) {
-    set_error("trnblas_mxfp4_dequantize: NULL or unaligned operand, or ldy smaller than K");
-    return TRNBLAS_ERR_ARG;
-  }
-  const dim3 grid(static_cast<unsigned>(ceil_div(rows, 32)), static_cast<unsigned>(ceil_div(K, 256)));
-  const int es = dtype == TRNBLAS_F32 ? 4 : 2;
-  const int vec = al16(Y) && (ldy * es) % 16 == 0;
-  const uint8_t* q = static_cast<const uint8_t*>(data);
-  const uint32_t* s = static_cast<const uint32_t*>(scales);
-  const int r = static_cast<int>(rows), k = static_cast<int>(K);
-  if (dtype == TRNBLAS_F32)
-    mxfp4_dequantize_kernel<float><<<grid, 256, 0, stream>>>(q, ldq, s, r, k, vec, static_cast<float*>(Y), ldy);
-  else if (dtype == TRNBLAS_BF16)
-    mxfp4_dequantize_kernel<__nv_bfloat16>
-        <<<grid, 256, 0, stream>>>(q, ldq, s, r, k, vec, static_cast<__nv_bfloat16*>(Y), ldy);
-  else
-    mxfp4_dequantize_kernel<__half><<<grid, 256, 0, stream>>>(q, ldq, s, r, k, vec, static_cast<__half*>(Y), ldy);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "mxfp4 dequantise kernel launch");
-}
-
-int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, float alpha,
-                       const void* A, int64_t lda, const void* scalesA, const void* B, int64_t ldb,
-                       const void* scalesB, const void* group_sizes, int sizes_64, float beta, const void* C,
-                       int64_t ldc, void* D, int64_t ldd, void* stream) {
+int check_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, const void* A, int64_t lda,
+                  const void* scalesA, const void* B, int64_t ldb, const void* scalesB, const void* group_sizes,
+                  float beta, const void* C, int64_t ldc, const void* D, int64_t ldd) {
   if (out_dtype != TRNBLAS_F32 && out_dtype != TRNBLAS_BF16 && out_dtype != TRNBLAS_F16) {
     set_error("trnblas_mxfp4_gemm: out_dtype must be F32, BF16 or F16");
     return TRNBLAS_ERR_ARG;
@@ -283,35 +294,234 @@ int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, i
     set_error("trnblas_mxfp4_gemm: NULL output, or ldc/ldd smaller than N");
     return TRNBLAS_ERR_ARG;
   }
-  if (K == 0 || groups == 0)
-    return trnblas_gemm(out_dtype, 1, rows, N, 0, alpha, nullptr, 1, 0, 0, nullptr, N, 0, 0, beta, C, ldc, 0,
-                        D, ldd, 0, nullptr, 0, stream);
+  if (K == 0 || groups == 0) return TRNBLAS_OK;
   if (int rc = check_mx("trnblas_mxfp4_gemm (A)", rows, K, lda)) return rc;
   if (int rc = check_mx("trnblas_mxfp4_gemm (B)", N, K, ldb)) return rc;
-  if (!A || !B || !scalesA || !scalesB || (reinterpret_cast<uintptr_t>(scalesA) & 3) ||
-      (reinterpret_cast<uintptr_t>(scalesB) & 3)) {
-    set_error("trnblas_mxfp4_gemm: NULL operand, or scales not on 4 bytes");
+  if (!A || !B || !scalesA || !scalesB || !al16(scalesA) || !al16(scalesB)) {
+    set_error("trnblas_mxfp4_gemm: NULL operand, or scales not on 16 bytes");
     return TRNBLAS_ERR_ARG;
   }
+  return TRNBLAS_OK;
+}
+
+}  // namespace
+}  // namespace tb
+
+namespace tb {
+namespace {
+
+// Thread blocks along K: enough for about 16 blocks an SM, at most one a chunk.
+unsigned k_blocks(long long xblocks, long long K) {
+  return static_cast<unsigned>(
+      std::max<long long>(1, std::min<long long>(ceil_div(K, 256), ceil_div(16ll * num_sms(), xblocks))));
+}
+
+template <bool GROUPED>
+int launch_quantize(int dtype, const GroupArgs& ga, long long blocks, int per_matrix, int64_t K, const void* X,
+                    int64_t ldx, void* data, int64_t ldq, void* scales, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(blocks * 4), k_blocks(blocks * 4, K));
+  const int vec = al16(X) && (ldx * (dtype == TRNBLAS_F32 ? 4 : 2)) % 16 == 0;
+  uint8_t* q = static_cast<uint8_t*>(data);
+  uint4* s = static_cast<uint4*>(scales);
+  const int k = static_cast<int>(K);
+  if (dtype == TRNBLAS_F32)
+    mxfp4_quantize_kernel<float, GROUPED>
+        <<<grid, 256, 0, stream>>>(static_cast<const float*>(X), ldx, ga, per_matrix, k, vec, q, ldq, s);
+  else if (dtype == TRNBLAS_BF16)
+    mxfp4_quantize_kernel<__nv_bfloat16, GROUPED>
+        <<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(X), ldx, ga, per_matrix, k, vec, q, ldq, s);
+  else
+    mxfp4_quantize_kernel<__half, GROUPED>
+        <<<grid, 256, 0, stream>>>(static_cast<const __half*>(X), ldx, ga, per_matrix, k, vec, q, ldq, s);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "mxfp4 quantise kernel launch");
+}
+
+bool kernel_dtype(int dtype) { return dtype == TRNBLAS_F32 || dtype == TRNBLAS_BF16 || dtype == TRNBLAS_F16; }
+
+int check_quantize(const char* what, int dtype, int64_t matrices, int64_t rows, int64_t K, const void* X, int64_t ldx,
+                   const void* data, int64_t ldq, const void* scales) {
+  const std::string w(what);
+  if (!kernel_dtype(dtype)) {
+    set_error(w + ": dtype must be F32, BF16 or F16");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (int rc = check_mx(what, rows, K, ldq)) return rc;
+  if (matrices < 0 || (matrices > 0 && matrices * ceil_div(rows, 128) > (1ll << 28))) {
+    set_error(w + ": too many rows");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (matrices == 0 || rows == 0 || K == 0) return TRNBLAS_OK;
+  if (!X || !data || !scales || ldx < K || !al16(data) || !al16(scales)) {
+    set_error(w + ": NULL or unaligned operand (16 bytes for data and scales), or a row stride smaller than K");
+    return TRNBLAS_ERR_ARG;
+  }
+  return TRNBLAS_OK;
+}
+
+size_t scale_bytes(int64_t rows, int64_t groups, int64_t K) {
+  return static_cast<size_t>(ceil_div(rows, 128) + groups) * ceil_div(K, 128) * 512;
+}
+
+// The product on data and scales in place; `grouped`: the rows' scales start a
+// block with every group.
+int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, float alpha, const void* A,
+                   int64_t lda, const void* scalesA, const void* B, int64_t ldb, const void* scalesB,
+                   const void* group_sizes, int sizes_64, float beta, const void* C, int64_t ldc, void* D,
+                   int64_t ldd, cudaStream_t stream) {
   const auto dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   const uint64_t kb = static_cast<uint64_t>(round_up(K, 32) / 2);
   // as for 16 bits: short row tiles and a deep pipeline where a group has at
-  // most 64 rows on average
+  // most 64 rows on average, CTA pairs above
   const bool small = rows <= 64 * groups;
-  CUtensorMap mw, mx, mx64;
+  const bool pair = !small && N > 128;
+  const uint64_t kw = static_cast<uint64_t>(ceil_div(K, 128));
+  const uint64_t wb = static_cast<uint64_t>(ceil_div(N, 128));
+  auto scale_map = [&](CUtensorMap* m, const void* base, uint64_t blocks, uint32_t box_blocks) {
+    const uint64_t dims[3] = {128, kw, blocks};
+    const uint64_t strides[2] = {128, 128 * kw};
+    const uint32_t box[3] = {128, 2, box_blocks};
+    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, base, 3, dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  CUtensorMap mw, mx, mxs, msw, msx;
   if (!encode_map_3d(&mw, dt, 1, B, kb, N, groups, ldb, ldb * N, 128, 128) ||
-      !encode_map_3d(&mx, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, small ? 64 : 192) ||
-      !encode_map_3d(&mx64, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, 64))
+      !encode_map_3d(&mx, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, small ? 64 : pair ? kMxPairBN / 2 : 192) ||
+      !encode_map_3d(&mxs, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, pair ? 32 : 64) ||
+      !scale_map(&msw, scalesB, wb * groups, 1) ||
+      !scale_map(&msx, scalesA, ceil_div(rows, 128) + (group_sizes ? groups : 0), small ? 1 : 2))
     return TRNBLAS_ERR_ALIGN;
   ExpertsParams p{};
   if (int rc = fill_experts(p, out_dtype, rows, groups, N, K, alpha, group_sizes, sizes_64, beta, C, ldc, D, ldd))
     return rc;
-  p.xs = static_cast<const uint32_t*>(scalesA);
-  p.xs_rows = rows;
-  p.ws = static_cast<const uint32_t*>(scalesB);
-  p.ws_rows = groups * N;
-  return small ? launch_experts<kExpMx4, 64>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream))
-               : launch_experts<kExpMx4, 192>(mw, mx, mx64, p, static_cast<cudaStream_t>(stream));
+  p.w_blocks = static_cast<int>(wb);
+  if (small) return launch_experts<kExpMx4, 64>(mw, mx, mxs, msw, msx, p, stream);
+  if (pair) return launch_experts_pair<kExpMx4, kMxPairBN>(mw, mx, mxs, msw, msx, p, stream);
+  return launch_experts<kExpMx4, 192>(mw, mx, mxs, msw, msx, p, stream);
+}
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" {
+
+int trnblas_mxfp4_quantize(int dtype, int64_t matrices, int64_t rows, int64_t K, const void* X, int64_t ldx,
+                           void* data, int64_t ldq, void* scales, void* stream) {
+  if (int rc = check_quantize("trnblas_mxfp4_quantize", dtype, matrices, rows, K, X, ldx, data, ldq, scales)) return rc;
+  if (matrices == 0 || rows == 0 || K == 0) return TRNBLAS_OK;
+  GroupArgs ga{};
+  ga.rows = static_cast<int>(rows);
+  const int per = static_cast<int>(ceil_div(rows, 128));
+  return launch_quantize<false>(dtype, ga, matrices * per, per, K, X, ldx, data, ldq, scales,
+                                static_cast<cudaStream_t>(stream));
+}
+
+int trnblas_mxfp4_dequantize(int dtype, int64_t matrices, int64_t rows, int64_t K, const void* data, int64_t ldq,
+                             const void* scales, void* Y, int64_t ldy, void* stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (int rc = check_quantize("trnblas_mxfp4_dequantize", dtype, matrices, rows, K, Y, ldy, data, ldq, scales))
+    return rc;
+  if (matrices == 0 || rows == 0 || K == 0) return TRNBLAS_OK;
+  const int per = static_cast<int>(ceil_div(rows, 128));
+  const long long blocks = matrices * per * 4;
+  const dim3 grid(static_cast<unsigned>(blocks), k_blocks(blocks, K));
+  const int vec = al16(Y) && (ldy * (dtype == TRNBLAS_F32 ? 4 : 2)) % 16 == 0;
+  const uint8_t* q = static_cast<const uint8_t*>(data);
+  const uint4* s = static_cast<const uint4*>(scales);
+  const int r = static_cast<int>(rows), k = static_cast<int>(K);
+  if (dtype == TRNBLAS_F32)
+    mxfp4_dequantize_kernel<float><<<grid, 256, 0, stream>>>(q, ldq, s, r, per, k, vec, static_cast<float*>(Y), ldy);
+  else if (dtype == TRNBLAS_BF16)
+    mxfp4_dequantize_kernel<__nv_bfloat16>
+        <<<grid, 256, 0, stream>>>(q, ldq, s, r, per, k, vec, static_cast<__nv_bfloat16*>(Y), ldy);
+  else
+    mxfp4_dequantize_kernel<__half><<<grid, 256, 0, stream>>>(q, ldq, s, r, per, k, vec, static_cast<__half*>(Y), ldy);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "mxfp4 dequantise kernel launch");
+}
+
+size_t trnblas_mxfp4_gemm_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped) {
+  if (rows <= 0 || groups <= 0 || K <= 0 || !grouped) return 0;
+  return scale_bytes(rows, groups, K);
+}
+
+int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, float alpha,
+                       const void* A, int64_t lda, const void* scalesA, const void* B, int64_t ldb,
+                       const void* scalesB, const void* group_sizes, int sizes_64, float beta, const void* C,
+                       int64_t ldc, void* D, int64_t ldd, void* workspace, size_t workspace_bytes,
+                       void* stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (int rc = check_mx_gemm(out_dtype, rows, groups, N, K, A, lda, scalesA, B, ldb, scalesB, group_sizes, beta, C,
+                             ldc, D, ldd))
+    return rc;
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  if (K == 0 || groups == 0)
+    return trnblas_gemm(out_dtype, 1, rows, N, 0, alpha, nullptr, 1, 0, 0, nullptr, N, 0, 0, beta, C, ldc, 0,
+                        D, ldd, 0, nullptr, 0, stream_);
+  if (group_sizes) {
+    if (!workspace || !al16(workspace) || workspace_bytes < scale_bytes(rows, groups, K)) {
+      set_error("trnblas_mxfp4_gemm: grouped needs " + std::to_string(scale_bytes(rows, groups, K)) +
+                " workspace bytes, 16-byte aligned");
+      return TRNBLAS_ERR_WORKSPACE;
+    }
+    GroupArgs ga{group_sizes, sizes_64, static_cast<int>(groups), static_cast<int>(rows), status_word()};
+    if (!ga.status) return TRNBLAS_ERR_CUDA;
+    const int kw = static_cast<int>(ceil_div(K, 128));
+    const dim3 grid(static_cast<unsigned>(ceil_div(rows, 128) + groups),
+                    static_cast<unsigned>(std::min<long long>(ceil_div(kw, 8), 65535)));
+    mxfp4_regroup_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint32_t*>(scalesA), ga, kw,
+                                                   static_cast<uint4*>(workspace));
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "mxfp4 regroup kernel launch");
+    scalesA = workspace;
+  }
+  return launch_mx_gemm(out_dtype, rows, groups, N, K, alpha, A, lda, scalesA, B, ldb, scalesB, group_sizes,
+                        sizes_64, beta, C, ldc, D, ldd, stream);
+}
+
+size_t trnblas_mxfp4_gemm_x_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped) {
+  if (rows <= 0 || groups <= 0 || K <= 0) return 0;
+  // packed values, then the scale blocks
+  return static_cast<size_t>(rows) * (round_up(K, 32) / 2) + scale_bytes(rows, grouped ? groups : 0, K);
+}
+
+int trnblas_mxfp4_gemm_x(int a_dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K,
+                         float alpha, const void* X, int64_t ldx, const void* B, int64_t ldb,
+                         const void* scalesB, const void* group_sizes, int sizes_64, float beta, const void* C,
+                         int64_t ldc, void* D, int64_t ldd, void* workspace, size_t workspace_bytes,
+                         void* stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (!kernel_dtype(a_dtype)) {
+    set_error("trnblas_mxfp4_gemm_x: a_dtype must be F32, BF16 or F16");
+    return TRNBLAS_ERR_ARG;
+  }
+  if (int rc = check_group_dims("trnblas_mxfp4_gemm_x", rows, groups, N, K)) return rc;
+  const int64_t ldq = round_up(K, 32) / 2;
+  uint8_t* data = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = data ? data + rows * ldq : nullptr;
+  if (rows == 0 || N == 0 || K == 0 || groups == 0)
+    return trnblas_mxfp4_gemm(out_dtype, rows, groups, N, K, alpha, X, ldq, X, B, ldb, scalesB, group_sizes, sizes_64,
+                              beta, C, ldc, D, ldd, workspace, workspace_bytes, stream_);
+  const size_t need = trnblas_mxfp4_gemm_x_workspace_size(rows, groups, K, group_sizes != nullptr);
+  if (!workspace || !al16(workspace) || workspace_bytes < need) {
+    set_error("trnblas_mxfp4_gemm_x: needs " + std::to_string(need) + " workspace bytes, 16-byte aligned");
+    return TRNBLAS_ERR_WORKSPACE;
+  }
+  if (int rc = check_mx_gemm(out_dtype, rows, groups, N, K, data, ldq, scales, B, ldb, scalesB, group_sizes, beta, C,
+                             ldc, D, ldd))
+    return rc;
+  if (int rc = check_quantize("trnblas_mxfp4_gemm_x", a_dtype, 1, rows, K, X, ldx, data, ldq, scales)) return rc;
+  GroupArgs ga{group_sizes, sizes_64, static_cast<int>(groups), static_cast<int>(rows), status_word()};
+  if (!ga.status) return TRNBLAS_ERR_CUDA;
+  const int per = static_cast<int>(ceil_div(rows, 128));
+  if (int rc = group_sizes
+                   ? launch_quantize<true>(a_dtype, ga, per + groups, per, K, X, ldx, data, ldq, scales, stream)
+                   : launch_quantize<false>(a_dtype, ga, per, per, K, X, ldx, data, ldq, scales, stream))
+    return rc;
+  return launch_mx_gemm(out_dtype, rows, groups, N, K, alpha, data, ldq, scales, B, ldb, scalesB, group_sizes,
+                        sizes_64, beta, C, ldc, D, ldd, stream);
 }
 
 }  // extern "C"

@@ -30,6 +30,12 @@ def _on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def _same_cuda_device(*ts) -> bool:
+    """Every tensor (or None) on one CUDA device: nothing to move."""
+    d = ts[0].get_device()
+    return d >= 0 and all(t is None or (isinstance(t, torch.Tensor) and t.get_device() == d) for t in ts)
+
+
 def _check_types(name: str, a, b, out_dtype):
     for x in (a, b):
         if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES:
@@ -68,26 +74,37 @@ def _rows_operand(x: torch.Tensor):
     return t, ld
 
 
+def _weights_operand(B: torch.Tensor, transB: bool):
+    """(tensor, ld, stored N x K, matrix stride) of the stack op(B) as `_flat_batch`
+    gives them; an ordinary contiguous stack needs no look at its strides."""
+    G, rows, cols = B.shape
+    if G > 1 and cols % 8 == 0 and cols and B.is_contiguous() and B.data_ptr() % 16 == 0:
+        return B, cols, transB, rows * cols
+    return _flat_batch(B.mT if transB else B, (G,), B.element_size(), False)
+
+
 def _c_operand(C, cols: int):
     """(tensor, ld) of a 2-D C whose rows are contiguous."""
     c = C if C.stride(-1) == 1 and C.stride(-2) >= cols else C.contiguous()
     return c, c.stride(-2)
 
 
-def _grouped(alpha, a, b, sizes, beta, C, out_dtype):
-    """alpha * a[r] @ b[g] (+ beta * C) on the kernel; C fusable or None."""
+def _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype):
+    """alpha * a[r] @ op(B[g]) (+ beta * C) on the kernel; C fusable or None."""
     rows, K = a.shape
-    G, _, Nn = b.shape
+    G = B.shape[0]
+    Nn = B.shape[1] if transB else B.shape[2]
     dev = a.device
     out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
     if rows == 0 or Nn == 0:
         return out
-    at, lda, bt, ldb, tb, sb = a, K, b, Nn, False, 0
+    at, lda, bt, ldb, tb, sb = a, K, B, Nn, False, 0
     if K and G:
         at, lda = _rows_operand(a)
-        bt, ldb, tb, sb = _flat_batch(b, (G,), b.element_size(), False)
+        bt, ldb, tb, sb = _weights_operand(B, transB)
     c_arg, ldc = _c_operand(C, Nn) if C is not None else (None, 0)
-    sizes = sizes.contiguous()
+    if not sizes.is_contiguous():
+        sizes = sizes.contiguous()
     with _on(dev):
         rc = N.lib().trnblas_grouped_gemm(
             N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(at), lda,
@@ -112,7 +129,8 @@ def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
     if C is not None:
         c_arg, ldc = _c_operand(C, Nn)
         sc = c_arg.stride(0)
-    sizes = sizes.contiguous()
+    if not sizes.is_contiguous():
+        sizes = sizes.contiguous()
     with _on(dev):
         rc = N.lib().trnblas_grouped_gemm_wgrad(
             N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, M, Nn, float(alpha), N.ptr(at), lda,
@@ -124,33 +142,31 @@ def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
 
 
 class _GroupedGemm(torch.autograd.Function):
-    """D[r] = alpha A[r] b[g] + beta C[r] with its gradients:
-    dA[r] = alpha dD[r] b[g]^T, db[g] = alpha A_g^T dD_g, dC = beta dD."""
+    """D[r] = alpha A[r] op(B[g]) + beta C[r] with its gradients:
+    dA[r] = alpha dD[r] op(B[g])^T, dB[g] = alpha A_g^T dD_g (or its transpose),
+    dC = beta dD."""
 
     @staticmethod
-    def forward(ctx, alpha, a, b, sizes, beta, C, out_dtype):
-        ctx.save_for_backward(a, b, sizes)
-        ctx.factors = (alpha, beta)
-        return _grouped(alpha, a, b, sizes, beta, C, out_dtype)
+    def forward(ctx, alpha, a, B, transB, sizes, beta, C, out_dtype):
+        ctx.save_for_backward(a, B, sizes)
+        ctx.args = (alpha, transB, beta)
+        return _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dD):
-        a, b, sizes = ctx.saved_tensors
-        alpha, beta = ctx.factors
-        y = dD.to(a.dtype)
-        da = db = dC = None
+        a, B, sizes = ctx.saved_tensors
+        alpha, transB, beta = ctx.args
+        y = dD if dD.dtype == a.dtype else dD.to(a.dtype)
+        da = dB = dC = None
         if ctx.needs_input_grad[1]:
-            da = _grouped(alpha, y, b.mT, sizes, 0.0, None, a.dtype)
+            da = _grouped(alpha, y, B, not transB, sizes, 0.0, None, a.dtype)
         if ctx.needs_input_grad[2]:
-            # in the layout of b's storage: b may be the transpose of what the caller holds
-            if b.stride(-2) == 1 and b.stride(-1) != 1:
-                db = _wgrad(alpha, y, a, sizes, 0.0, None, b.dtype).mT
-            else:
-                db = _wgrad(alpha, a, y, sizes, 0.0, None, b.dtype)
-        if ctx.needs_input_grad[5]:
+            l, r = (y, a) if transB else (a, y)
+            dB = _wgrad(alpha, l, r, sizes, 0.0, None, B.dtype)
+        if ctx.needs_input_grad[6]:
             dC = beta * dD
-        return None, da, db, None, None, dC, None
+        return None, da, dB, None, None, None, dC, None
 
 
 def grouped_gemm(
@@ -186,21 +202,23 @@ def grouped_gemm(
     out_dtype = _check_types(name, A, B, out_dtype)
     if A.dim() != 2 or B.dim() != 3:
         raise ValueError(f"{name}: A is 2-D and B 3-D, got {tuple(A.shape)} and {tuple(B.shape)}")
-    b = B.mT if transB else B
-    if A.shape[1] != b.shape[1]:
-        raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, op(B) {tuple(b.shape)}")
-    check_group_sizes(name, group_sizes, b.shape[0], A.shape[0])
+    if A.shape[1] != B.shape[2 if transB else 1]:
+        raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, B {tuple(B.shape)}, transB={transB}")
+    check_group_sizes(name, group_sizes, B.shape[0], A.shape[0])
+    grad = torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)
+    if not grad and C is None and _same_cuda_device(A, B, group_sizes):
+        return _grouped(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)
-    a, b, sizes, Cd = _to(A, dev), _to(b, dev), _to(group_sizes, dev), _to(C, dev)
-    fuse = _fuse_c(Cd, beta, (a.shape[0], b.shape[2]), out_dtype, dev)
+    a, b, sizes, Cd = _to(A, dev), _to(B, dev), _to(group_sizes, dev), _to(C, dev)
+    fuse = _fuse_c(Cd, beta, (a.shape[0], b.shape[1] if transB else b.shape[2]), out_dtype, dev)
     c_arg = Cd if fuse else None
-    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or (fuse and Cd.requires_grad)):
-        r = _GroupedGemm.apply(alpha, a, b, sizes, beta, c_arg, out_dtype)
+    if grad or (torch.is_grad_enabled() and fuse and Cd.requires_grad):
+        r = _GroupedGemm.apply(alpha, a, b, transB, sizes, beta, c_arg, out_dtype)
         if not fuse and C is not None and beta != 0.0:
             r = r + beta * Cd
         return r if home == dev else r.to(home)
-    r = _grouped(alpha, a, b, sizes, beta, c_arg, out_dtype)
+    r = _grouped(alpha, a, b, transB, sizes, beta, c_arg, out_dtype)
     if not fuse:
         r = _add_c(r, beta, Cd)
     return _home(r, home, dev)
@@ -228,6 +246,8 @@ def grouped_gemm_wgrad(
     if A.dim() != 2 or B.dim() != 2 or A.shape[0] != B.shape[0]:
         raise ValueError(f"{name}: A and B are 2-D with the same rows, got {tuple(A.shape)} and {tuple(B.shape)}")
     check_group_sizes(name, group_sizes, None, A.shape[0])
+    if C is None and _same_cuda_device(A, B, group_sizes):
+        return _wgrad(alpha, A, B, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)
     a, b, sizes, Cd = (_to(A.detach(), dev), _to(B.detach(), dev), _to(group_sizes, dev),

@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _native as N
-from .experts import _c_operand, _on, check_group_sizes
+from .experts import _c_operand, _on, _same_cuda_device, check_group_sizes
 from .level3 import _add_c, _cuda_device, _fuse_c, _home, _to
 
 BLOCK = 32
@@ -27,9 +27,10 @@ class MXFP4Tensor:
 
     data    uint8 (..., rows, round_up(K, 32) / 2): two values a byte, the even
             one in the low half, zero behind K;
-    scales  uint8 (ceil(K / 128), all rows, 4): the E8M0 bytes of a row's four
-            blocks in 128 values; what a tensor-core tile reads is contiguous
-            whatever row it starts at;
+    scales  uint8 (matrices, ceil(rows / 128), ceil(K / 128), 512), matrices the
+            product of the leading dimensions: the E8M0 bytes of 128 rows x 128
+            values, the four of row r at 16 * (r % 32) + 4 * (r / 32 % 4), as the
+            tensor cores take them; zero behind the rows and behind K;
     shape   the logical shape.
     """
 
@@ -43,7 +44,7 @@ class MXFP4Tensor:
         want = (*lead, _round_up(K, BLOCK) // 2)
         if data.dtype != torch.uint8 or tuple(data.shape) != want or not data.is_contiguous():
             raise ValueError(f"MXFP4Tensor: data must be contiguous uint8 {want}, got {data.dtype} {tuple(data.shape)}")
-        want = (-(-K // 128), math.prod(lead), 4)
+        want = _scale_shape(self.shape)
         if scales.dtype != torch.uint8 or tuple(scales.shape) != want or not scales.is_contiguous():
             raise ValueError(
                 f"MXFP4Tensor: scales must be contiguous uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
@@ -79,18 +80,21 @@ class MXFP4Tensor:
         data[..., :kb] = codes[..., :kb]
         if K % 2:
             data[..., kb - 1] &= 0x0F
-        kw = -(-K // 128)
-        rows = math.prod(lead)
-        words = scales.new_zeros((rows, 4 * kw))
-        words[:, :nb] = scales.reshape(rows, nb)
-        return cls(data, words.view(rows, kw, 4).transpose(0, 1).contiguous(), (*lead, K))
+        mats, rb, kw, _ = _scale_shape((*lead, K))
+        rows = lead[-1]
+        words = scales.new_zeros((mats, rb * 128, 4 * kw))
+        words[:, :rows, :nb] = scales.reshape(mats, rows, nb)
+        # (block, row / 32, row % 32, K block, byte) -> (block, K block, row % 32, row / 32, byte)
+        blocks = words.view(mats, rb, 4, 32, kw, 4).permute(0, 1, 4, 3, 2, 5)
+        return cls(data, blocks.reshape(mats, rb, kw, 512), (*lead, K))
 
     def parts(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(codes, scales) in row order, as `from_parts` takes them."""
         *lead, K = self.shape
-        rows, nb = math.prod(lead), -(-K // BLOCK)
-        s = self.scales.transpose(0, 1).reshape(rows, -1)[:, :nb]
-        return self.data.clone(), s.reshape(*lead, nb).clone()
+        mats, rb, kw, _ = self.scales.shape
+        words = self.scales.view(mats, rb, kw, 32, 4, 4).permute(0, 1, 4, 3, 2, 5).reshape(mats, rb * 128, 4 * kw)
+        nb = -(-K // BLOCK)
+        return self.data.clone(), words[:, : lead[-1], :nb].reshape(*lead, nb).clone()
 
     def __repr__(self) -> str:
         return f"MXFP4Tensor(shape={tuple(self.shape)}, device={self.device})"
@@ -100,24 +104,45 @@ def _round_up(a: int, b: int) -> int:
     return -(-a // b) * b
 
 
+def _scale_shape(shape):
+    """Shape of the scale blocks of a (..., rows, K) operand."""
+    return math.prod(shape[:-2]), -(-shape[-2] // 128), -(-shape[-1] // 128), 512
+
+
+def _rows2d(x: torch.Tensor):
+    """(tensor, ldx, rows, K) of x (..., rows, K): values along K contiguous."""
+    K = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(math.prod(x.shape[:-1]), K)
+    rows = x.shape[0]
+    s0, s1 = x.stride()
+    if (s1 != 1 and K > 1) or (rows > 1 and s0 < K):
+        x, s0 = x.contiguous(), K
+    return x, max(s0, K), rows, K
+
+
+def _unchecked(data, scales, shape) -> MXFP4Tensor:
+    """An MXFP4Tensor of this module's own making."""
+    q = object.__new__(MXFP4Tensor)
+    q.data, q.scales, q.shape = data, scales, shape
+    return q
+
+
 def _quantize(x: torch.Tensor) -> MXFP4Tensor:
     """x (..., rows, K) on a CUDA device."""
-    *lead, K = x.shape
-    rows = math.prod(lead)
-    x2 = x.detach().reshape(rows, K)
-    if K and x2.stride(1) != 1 and K > 1 or (rows > 1 and x2.stride(0) < K):
-        x2 = x2.contiguous()
+    x2, ldx, rows, K = _rows2d(x)
+    lead = x.shape[:-1]
     ldq = _round_up(K, BLOCK) // 2
     data = torch.empty((*lead, ldq), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((-(-K // 128), rows, 4), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_shape(x.shape), dtype=torch.uint8, device=x.device)
     if rows and K:
         with _on(x.device):
             rc = N.lib().trnblas_mxfp4_quantize(
-                N.dtype_code(x.dtype), rows, K, N.ptr(x2), max(x2.stride(0), K), N.ptr(data), ldq, N.ptr(scales),
+                N.dtype_code(x.dtype), scales.shape[0], x.shape[-2], K, N.ptr(x2), ldx, N.ptr(data), ldq, N.ptr(scales),
                 N.stream_ptr(x.device))
         N.check(rc, "trnblas_mxfp4_quantize")
         N.count_launches(1)
-    return MXFP4Tensor(data, scales, x.shape)
+    return _unchecked(data, scales, x.shape)
 
 
 def quantize_mxfp4(x: torch.Tensor) -> MXFP4Tensor:
@@ -133,6 +158,8 @@ def quantize_mxfp4(x: torch.Tensor) -> MXFP4Tensor:
         raise TypeError(f"quantize_mxfp4: a float32, bfloat16 or float16 tensor, got {getattr(x, 'dtype', type(x))}")
     if x.dim() < 2:
         raise ValueError(f"quantize_mxfp4: a tensor (..., rows, K), got {tuple(x.shape)}")
+    if x.is_cuda:
+        return _quantize(x)
     dev = _cuda_device(x)
     q = _quantize(_to(x, dev))
     return q if x.device == dev else q.to(x.device)
@@ -145,21 +172,20 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.float32) -> torc
         raise TypeError(f"dequantize_mxfp4: an MXFP4Tensor, got {type(q)}")
     if dtype not in _OUT:
         raise TypeError(f"dequantize_mxfp4: dtype is float32, bfloat16 or float16, got {dtype}")
-    home = q.device
-    dev = _cuda_device(q.data)
-    if home != dev:
+    home = dev = q.device
+    if not q.data.is_cuda:
+        dev = _cuda_device(q.data)
         q = q.to(dev)
-    *lead, K = q.shape
-    rows = math.prod(lead)
+    K = q.shape[-1]
     out = torch.empty(tuple(q.shape), dtype=dtype, device=dev)
     if out.numel():
         with _on(dev):
             rc = N.lib().trnblas_mxfp4_dequantize(
-                N.dtype_code(dtype), rows, K, N.ptr(q.data), q.data.shape[-1], N.ptr(q.scales), N.ptr(out), K,
+                N.dtype_code(dtype), q.scales.shape[0], q.shape[-2], K, N.ptr(q.data), q.data.shape[-1], N.ptr(q.scales), N.ptr(out), K,
                 N.stream_ptr(dev))
         N.check(rc, "trnblas_mxfp4_dequantize")
         N.count_launches(1)
-    return _home(out, home, dev)
+    return out if home == dev else _home(out, home, dev)
 
 
 def _operands(name, A, B, b_dim, out_dtype):
@@ -176,35 +202,50 @@ def _operands(name, A, B, b_dim, out_dtype):
 
 
 def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
-    home = A.device
-    dev = _cuda_device(A if isinstance(A, torch.Tensor) else A.data, B.data, C, sizes)
-    if B.device != dev:
-        B = B.to(dev)
-    if isinstance(A, MXFP4Tensor):
-        qa = A if A.device == dev else A.to(dev)
+    quantised = isinstance(A, MXFP4Tensor)
+    a = A.data if quantised else A
+    if _same_cuda_device(a, B.data, sizes, C):
+        home = dev = a.device
     else:
-        qa = _quantize(_to(A, dev))
-    sizes, Cd = _to(sizes, dev), _to(C, dev)
+        home = A.device
+        dev = _cuda_device(a, B.data, C, sizes)
+        if B.device != dev:
+            B = B.to(dev)
+        if A.device != dev:
+            A = A.to(dev)
+        sizes, C = _to(sizes, dev), _to(C, dev)
     rows, K = A.shape
     Nn = B.shape[-2]
     G = B.shape[0] if sizes is not None else 1
     out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
-    fuse = _fuse_c(Cd, beta, out.shape, out_dtype, dev)
-    if out.numel():
-        c_arg, ldc = _c_operand(Cd.detach(), Nn) if fuse else (None, 0)
-        if sizes is not None:
+    fuse = _fuse_c(C, beta, out.shape, out_dtype, dev)
+    if rows and Nn:
+        c_arg, ldc = _c_operand(C, Nn) if fuse else (None, 0)
+        if sizes is not None and not sizes.is_contiguous():
             sizes = sizes.contiguous()
-        with _on(dev):
-            rc = N.lib().trnblas_mxfp4_gemm(
-                N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(qa.data), qa.data.shape[-1],
-                N.ptr(qa.scales), N.ptr(B.data), B.data.shape[-1], N.ptr(B.scales), N.ptr(sizes),
+        tail = (N.ptr(B.data), B.data.shape[-1], N.ptr(B.scales), N.ptr(sizes),
                 int(sizes is not None and sizes.dtype == torch.int64), float(beta) if fuse else 0.0, N.ptr(c_arg),
-                ldc, N.ptr(out), Nn, N.stream_ptr(dev))
+                ldc, N.ptr(out), Nn)
+        with _on(dev):
+            # scale blocks of 128 rows; with groups, a block starts with each
+            sf_bytes = (-(-rows // 128) + (G if sizes is not None else 0)) * -(-K // 128) * 512
+            if quantised:
+                ws = N.workspace(sf_bytes if sizes is not None else 0, dev)
+                rc = N.lib().trnblas_mxfp4_gemm(
+                    N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(A.data), A.data.shape[-1],
+                    N.ptr(A.scales), *tail, N.ptr(ws), sf_bytes, N.stream_ptr(dev))
+            else:
+                x, ldx, _, _ = _rows2d(A)
+                ws_bytes = rows * (_round_up(K, BLOCK) // 2) + sf_bytes
+                ws = N.workspace(ws_bytes, dev)
+                rc = N.lib().trnblas_mxfp4_gemm_x(
+                    N.dtype_code(x.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(x), ldx,
+                    *tail, N.ptr(ws), ws_bytes, N.stream_ptr(dev))
         N.check(rc, name)
-        N.count_launches(1)
+        N.count_launches(1 if (quantised and sizes is None) or not K or not G else 2)
     if not fuse:
-        out = _add_c(out, beta, Cd.detach() if isinstance(Cd, torch.Tensor) else Cd)
-    return _home(out, home, dev)
+        out = _add_c(out, beta, C.detach() if isinstance(C, torch.Tensor) else C)
+    return out if home == dev else _home(out, home, dev)
 
 
 def gemm_mxfp4(
