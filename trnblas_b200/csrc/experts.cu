@@ -113,15 +113,13 @@ int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t g
     set_error("trnblas_grouped_gemm_wgrad: NULL operand, or lda/ldb smaller than the row length");
     return TRNBLAS_ERR_ARG;
   }
-  using Cfg = WgradCfg;
   const auto dt = dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap ma, mb;
-  if (!encode_map_3d(&ma, dt, 2, A, M, rows, 1, lda, round_up(lda * rows, 8), 64, 64) ||
-      !encode_map_3d(&mb, dt, 2, B, N, rows, 1, ldb, round_up(ldb * rows, 8), 64, 64))
-    return TRNBLAS_ERR_ALIGN;
+  // CTA pairs (256 x 256 tiles) where both sides have columns for two CTAs
+  const bool pair = M > 128 && N > 128;
+  const int bm = pair ? WgradPairCfg::BM : WgradCfg::BM, bn = pair ? WgradPairCfg::BN : WgradCfg::BN;
   WgradParams w{};
-  w.p.tiles_m = static_cast<int>(ceil_div(M, Cfg::BM));
-  w.p.tiles_n = static_cast<int>(ceil_div(N, Cfg::BN));
+  w.p.tiles_m = static_cast<int>(ceil_div(M, bm));
+  w.p.tiles_n = static_cast<int>(ceil_div(N, bn));
   const long long tiles = groups * static_cast<long long>(w.p.tiles_m) * w.p.tiles_n;
   if (tiles > (1ll << 30)) {
     set_error("trnblas_grouped_gemm_wgrad: too many tiles");
@@ -148,12 +146,48 @@ int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t g
   w.sizes = group_sizes;
   w.sizes64 = sizes_64;
   w.in_fmt = dtype == TRNBLAS_BF16 ? kFmtBF16 : kFmtF16;
-  static bool attr_set[64] = {};
-  if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_kernel), Cfg::SMEM, attr_set)) return rc;
-  const int grid = static_cast<int>(std::min<long long>(tiles, num_sms()));
-  wgrad_kernel<<<grid, Cfg::THREADS, Cfg::SMEM, static_cast<cudaStream_t>(stream_)>>>(ma, mb, w);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "weight gradient kernel launch");
+  // whole blocks of 64 columns: a map of 64 columns x rows x blocks, so that one
+  // copy brings 128 columns
+  w.wide = pair && M % 64 == 0 && N % 64 == 0;
+  CUtensorMap ma, mb, md;
+  auto rows_map = [&](CUtensorMap* m, const void* X, int64_t cols, int64_t ld) {
+    if (!w.wide) return encode_map_3d(m, dt, 2, X, cols, rows, 1, ld, round_up(ld * rows, 8), 64, 64);
+    const uint64_t dims[3] = {64, static_cast<uint64_t>(rows), static_cast<uint64_t>(cols / 64)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(ld), 64};
+    const uint32_t box[3] = {64, 64, 2};
+    return encode_map(m, dt, 2, X, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (!rows_map(&ma, A, M, lda) || !rows_map(&mb, B, N, ldb)) return TRNBLAS_ERR_ALIGN;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  static bool attr_set[64] = {}, pair_attr_set[64] = {};
+  if (!pair) {
+    if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_kernel), WgradCfg::SMEM, attr_set)) return rc;
+    const int grid = static_cast<int>(std::min<long long>(tiles, num_sms()));
+    wgrad_kernel<<<grid, WgradCfg::THREADS, WgradCfg::SMEM, stream>>>(ma, mb, w);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "weight gradient kernel launch");
+  }
+  // stores by TMA where D's rows lie on 16 bytes and no C is added
+  const int oes = out_dtype == TRNBLAS_F32 ? 4 : 2;
+  const int64_t sd = groups > 1 ? strideD : round_up(ldd * M, 8);
+  w.tma_d = !has_c && (reinterpret_cast<uintptr_t>(D) & 15) == 0 && (ldd * oes) % 16 == 0 && (sd * oes) % 16 == 0;
+  md = ma;
+  if (w.tma_d && !encode_map_3d(&md,
+                                out_dtype == TRNBLAS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : out_dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                oes, D, N, M, groups, ldd, sd, 128 / oes, 32))
+    return TRNBLAS_ERR_ALIGN;
+  if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_pair_kernel), WgradPairCfg::SMEM, pair_attr_set))
+    return rc;
+  static int max_pairs[64] = {};
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = pair_config(attr, WgradPairCfg::THREADS, WgradPairCfg::SMEM, stream);
+  int pairs = 0;
+  if (int rc = resident_pairs(wgrad_pair_kernel, cfg, max_pairs, pairs)) return rc;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<long long>(tiles, pairs)), 1, 1);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, wgrad_pair_kernel, ma, mb, md, static_cast<const WgradParams>(w));
+  return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "weight gradient pair kernel launch");
 }
 
 }  // extern "C"

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
     uint32_t phase = 0;
     const bool aborted = [&] {
     for (int t = pair; t < work_tiles; t += npairs) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, t);
       const int half = ((e.nv + 31) & ~31) / 2;  // rows of each CTA
       // above three quarters one full box, else boxes of 32 rows
       const int boxes = half > Cfg::HN * 3 / 4 ? 0 : (half + 31) / 32;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
     uint32_t phase = 0;
     long long g0 = 0;  // K blocks issued before this tile
     for (int t = pair; t < work_tiles; t += npairs, ++tc) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, t);
       const uint32_t nm = warp_uniform(static_cast<uint32_t>((e.nv + 31) & ~31));
       const uint32_t xcol = warp_uniform(static_cast<uint32_t>(e.x0 >> 5) & 3u);  // in its scale block
       const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) + (1u << 27)  // M = 256
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
     const uint32_t acce_leader = mapa_shared(smem_u32(acce_bar), 0);
     int tc = 0;
     for (int t = pair; t < num_tiles; t += npairs) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, t);
       const int n0 = e.n0 + 128 * rank + 32 * q;
       if (t >= work_tiles) {
         float z[32];

@@ -145,11 +145,16 @@ struct ExpTile {
   int x0;      // first row within the group
 };
 
-// Tile t: the tiles of one weight block are next to one another, so the CTAs
-// that run together share it and the group's rows. BN: most rows of a tile, a
-// multiple of STEP; WT: weight columns of a tile.
+// Tile t of the walk: within a group, bands of at most kBand row tiles; in a
+// band, the row tiles of one weight block next to one another. The CTAs that
+// run together then share a few weight blocks and a band's rows, and a long
+// group's rows are not read from DRAM once for every weight block (16384 rows
+// in one group, K = N = 4096: bands of 8 against none, see the kernels' figures). BN: most rows of
+// a tile, a multiple of STEP; WT: weight columns of a tile.
+constexpr int kBand = 8;
+
 template <int BN, int STEP = 16, int WT = 128>
-__device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, int t) {
+__device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, int tiles_w, int t) {
   int lo = 0, hi = groups + 1;  // tile0[lo] <= t < tile0[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -164,7 +169,9 @@ __device__ __forceinline__ ExpTile exp_tile(const GroupTable& tb, int groups, in
   // never empty, since nt - 1 tiles of at most BN rows do not cover m)
   const int step = ((m + nt - 1) / nt + STEP - 1) & ~(STEP - 1);
   const int i = t - tb.tile0[lo];
-  const int w = i / nt, x = i - w * nt;
+  const int band = i / (kBand * tiles_w), j = i - band * kBand * tiles_w;
+  const int width = min(kBand, nt - band * kBand);
+  const int w = j / width, x = band * kBand + j - w * width;
   e.x0 = x * step;
   e.r0 = first + e.x0;
   e.nv = min(step, m - x * step);
@@ -361,7 +368,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     uint32_t phase = 0;
     const bool aborted = [&] {
     for (int t = blockIdx.x; t < work_tiles; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
       // above three quarters of the tile one full box, else boxes of 64 rows
       const int boxes = (BN == 64 || e.nv > BN * 3 / 4) ? 0 : (e.nv + 63) / 64;
       const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * 64 * 128 : Cfg::X_TILE);
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     int stage = 0, tc = 0;
     uint32_t phase = 0;
     for (int t = blockIdx.x; t < work_tiles; t += gridDim.x, ++tc) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
       const uint32_t nm = warp_uniform(static_cast<uint32_t>((e.nv + 15) & ~15));
       const uint32_t xcol = warp_uniform(static_cast<uint32_t>(e.x0 >> 5) & 3u);  // in its scale block
       const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn, 0, 128, nm);
@@ -500,7 +507,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     int tc = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, t);
+      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
       const int n0 = e.n0 + 32 * q;
       if (t >= work_tiles) {
         float z[32];

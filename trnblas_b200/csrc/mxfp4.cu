@@ -9,8 +9,6 @@
 //           the word of a row's four E8M0 bytes (zero past K) at 16 * (r % 32)
 //           + 4 * (r / 32 % 4), as the tensor core's copy wants them. Every
 //           matrix of a stack starts a block of its own.
-#include <cuda_fp4.h>
-
 #include <algorithm>
 
 #include "experts_host.hpp"
@@ -18,66 +16,108 @@
 namespace tb {
 namespace {
 
+// Eight neighbouring values of a row as they are stored.
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, int valid, bool vec, float (&x)[8]) {
-  if (valid <= 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    return;
-  }
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* src, int valid, bool vec) {
+  Raw8<T> r;
+  constexpr int V = static_cast<int>(sizeof(T)) / 2;
   if (vec && valid >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(src));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
-        }
-      }
-    }
-    return;
+    for (int i = 0; i < V; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    return r;
+  }
+  uint32_t w[4 * V] = {};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid)
+        w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(src) + i)) << (16 * (i & 1));
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < valid ? static_cast<float>(src[i]) : 0.0f;
+  for (int i = 0; i < V; ++i) r.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  return r;
+}
+
+// 8 E2M1 codes of 8 floats, the first in the lowest bits: nearest, ties to
+// even, saturating at 6.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&u)[8]) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(u[0]), "f"(u[1]), "f"(u[2]), "f"(u[3]), "f"(u[4]), "f"(u[5]), "f"(u[6]), "f"(u[7]));
+  return w;
 }
 
 // Four lanes hold a block of 32 (8 values each). The block's unit is 2^(s - 127)
-// with s = max(E, 2) - 2, E the biased exponent of the block's largest
+// with s = max(E, 2) - 2, E the biased fp32 exponent of the block's largest
 // magnitude: the largest power of two not above it, divided by 4 (E2M1's
 // largest power of two). Scaling by it is exact; the conversion rounds to the
 // nearest of 0, .5, 1, 1.5, 2, 3, 4, 6, ties to even, and saturates (a block's
 // largest magnitude is below 8 units). A block that holds an infinity or a NaN
-// gets the NaN scale 255.
-__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& s) {
-  uint32_t m = 0;
+// gets the NaN scale 255. The maximum is taken on the magnitudes' bits, which
+// order as the values do (16-bit types: two at a time).
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(const Raw8<T>& r, uint32_t& s) {
+  float x[8];
+  uint32_t E;
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t w[8] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w, r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t E = m >> 23;
-  if (E == 255) {
-    s = 255;
-    return 0;
+    for (int i = 0; i < 8; ++i) {
+      m = max(m, w[i] & 0x7FFFFFFFu);
+      x[i] = __uint_as_float(w[i]);
+    }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    E = m >> 23;
+  } else {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    uint32_t m = __vimax3_u16x2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu, w[2] & 0x7FFF7FFFu);
+    uint32_t o = __shfl_xor_sync(0xffffffffu, m = __vimax3_u16x2(m, w[3] & 0x7FFF7FFFu, 0u), 1);
+    m = __vimax3_u16x2(m, o, 0u);
+    o = __shfl_xor_sync(0xffffffffu, m, 2);
+    m = __vimax3_u16x2(m, o, 0u);
+    m = max(m & 0xFFFFu, m >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      E = m >> 7;
+    else
+      E = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m)))) >> 23;
   }
   s = max(E, 2u) - 2u;
   const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s), normal
-  uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv),
-                                                        __NV_E2M1, cudaRoundNearest))
-         << (8 * i);
+  for (int i = 0; i < 8; ++i) x[i] *= inv;
+  uint32_t w = e2m1x8(x);
+  if (E == 255) {
+    s = 255;
+    w = 0;
+  }
   return w;
 }
 
@@ -148,15 +188,22 @@ __global__ void __launch_bounds__(256)
     ok[i] = l0 + 32 * i < br.limit;
     row[i] = ok[i] ? br.base + l0 + 32 * i : br.base;
   }
-  for (int k = blockIdx.y * 256 + lane * 8; k - lane * 8 < K; k += gridDim.y * 256) {
-    float x[4][8];
+  const int kstep = gridDim.y * 256;
+  int k = blockIdx.y * 256 + lane * 8;
+  Raw8<T> cur[4], nxt[4];
+  auto fetch = [&](Raw8<T> (&dst)[4], int at) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load8(X + row[i] * ldx + (k < K ? k : 0), ok[i] ? K - k : 0, vec, x[i]);
+    for (int i = 0; i < 4; ++i)
+      dst[i] = load8(X + row[i] * ldx + (at < K ? at : 0), ok[i] ? K - at : 0, vec);
+  };
+  fetch(cur, k);
+  for (; k - lane * 8 < K; k += kstep) {
+    if (k - lane * 8 + kstep < K) fetch(nxt, k + kstep);  // in flight while this chunk is converted
     uint32_t word[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t s;
-      const uint32_t w = quantize8(x[i], s);
+      const uint32_t w = quantize8<T>(cur[i], s);
       if (ok[i] && (k >> 1) < ldq) *reinterpret_cast<uint32_t*>(data + row[i] * ldq + (k >> 1)) = w;
       // the four scale bytes of 16 lanes; zero past K's last block
       if ((k & ~31) >= K || !ok[i]) s = 0;
@@ -169,6 +216,8 @@ __global__ void __launch_bounds__(256)
     if ((lane & 15) == 0 && kw < kwords)
       scales[(static_cast<long long>(blk) * kwords + kw) * 32 + l32] =
           make_uint4(word[0], word[1], word[2], word[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
   }
 }
 
@@ -194,20 +243,45 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T to_out(float v);
-template <>
-__device__ __forceinline__ float to_out<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half to_out<__half>(float v) { return __float2half_rn(v); }
+// Two E2M1 codes (the low byte of c, the earlier in its low half) as bf16 bits:
+// a code s ee m is the bf16 number with these bits at the sign, the low
+// exponent and the top mantissa places, times 2^126 (subnormals included), so no
+// table is read.
+__device__ __forceinline__ uint32_t e2m1x2_bits(uint32_t c) {
+  const uint32_t y = (c & 0xFu) | ((c & 0xF0u) << 12);
+  return ((y & 0x00070007u) << 6) | ((y & 0x00080008u) << 12);
+}
 
-// The values: 8 a lane, 4 rows a warp as above. An E2M1 code s ee m is the
-// fp16 number with these bits at the sign, the low exponent and the top
-// mantissa places, times 2^14 (subnormals included), so no table is read. The
-// unit 2^(s - 127) is subnormal for s = 0 and NaN for s = 255; the product of
-// a 2-bit mantissa and a power of two is exact, and rounds once to T.
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+
+// 8 values of codes w in units of 2^(s - 127). bf16 holds every product of a
+// 2-bit mantissa and a power of two down to 2^-133 exactly, so the two
+// multiplications (by 2^126, by the unit: subnormal for s = 0, NaN for s = 255)
+// are exact in pairs of bf16; fp32 and fp16 are taken from there, fp16 with its
+// own rounding. (Units above 2^125 overflow to infinities where fp32 does.)
+template <typename T>
+__device__ __forceinline__ void dequantize8(uint32_t w, uint32_t s, T (&out)[8]) {
+  const uint32_t ub = s == 255 ? 0x7FC0u : (s == 0 ? 0x0040u : s << 7);
+  const __nv_bfloat162 unit = as_bf162(ub | (ub << 16)), big = as_bf162(0x7E807E80u);  // 2^126
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 v = __hmul2(__hmul2(as_bf162(e2m1x2_bits((w >> (8 * j)) & 0xFFu)), big), unit);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      reinterpret_cast<__nv_bfloat162*>(out)[j] = v;
+    } else {
+      const float2 f = __bfloat1622float2(v);
+      if constexpr (std::is_same<T, float>::value) {
+        out[2 * j] = f.x;
+        out[2 * j + 1] = f.y;
+      } else {
+        out[2 * j] = __float2half_rn(f.x);
+        out[2 * j + 1] = __float2half_rn(f.y);
+      }
+    }
+  }
+}
+
+// 8 values a lane, 4 rows a warp as in the quantiser. Bounded by the write.
 template <typename T>
 __global__ void __launch_bounds__(256)
     mxfp4_dequantize_kernel(const uint8_t* __restrict__ data, long long ldq,
@@ -233,16 +307,8 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 4; ++i) {
       if (l0 + 32 * i >= br.limit) break;
       const uint32_t s = (sw[i] >> (8 * ((k >> 5) & 3))) & 0xFFu;
-      const float unit = s == 255 ? __uint_as_float(0x7FC00000u)
-                                  : (s == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23));
-      T out[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t c = (w[i] >> (4 * j)) & 0xFu;
-        const float v =
-            __half2float(__ushort_as_half(static_cast<unsigned short>(((c & 8u) << 12) | ((c & 7u) << 9))));
-        out[j] = to_out<T>(v * 16384.0f * unit);
-      }
+      alignas(16) T out[8];
+      dequantize8<T>(w[i], s, out);
       T* dst = Y + (br.base + l0 + 32 * i) * ldy + k;
       if (vec && k + 8 <= K) {
 #pragma unroll
@@ -310,10 +376,12 @@ int check_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_
 namespace tb {
 namespace {
 
-// Thread blocks along K: enough for about 16 blocks an SM, at most one a chunk.
+// Thread blocks along K: about four chunks of 256 each, so that a block has the
+// next chunk in flight behind the one it converts; one each where that leaves
+// less than two blocks an SM.
 unsigned k_blocks(long long xblocks, long long K) {
-  return static_cast<unsigned>(
-      std::max<long long>(1, std::min<long long>(ceil_div(K, 256), ceil_div(16ll * num_sms(), xblocks))));
+  const long long chunks = ceil_div(K, 256), y = ceil_div(chunks, 4);
+  return static_cast<unsigned>(std::min<long long>(xblocks * y < 2ll * num_sms() ? chunks : y, 65535));
 }
 
 template <bool GROUPED>
