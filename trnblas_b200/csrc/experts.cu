@@ -65,7 +65,7 @@ int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups,
   // are weight columns for both.
   const bool small = rows <= 48 * groups;
   const bool pair = !small && N > 128;
-  const bool wide = pair && !transB && N % 64 == 0;  // both 64-column blocks in one copy
+  const bool wide = !transB && N % 64 == 0;  // both 64-column blocks in one copy
   CUtensorMap mw, mx, mxs;
   bool ok;
   if (transB) {
@@ -79,7 +79,7 @@ int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups,
     ok = encode_map_3d(&mw, dt, 2, B, N, K, nb, ldb, sb, 64, 64);
   }
   ok = ok && encode_map_3d(&mx, dt, 2, A, K, rows, 1, lda, sa, 64, pair ? 128 : small ? 64 : 256) &&
-       encode_map_3d(&mxs, dt, 2, A, K, rows, 1, lda, sa, 64, pair ? 32 : 64);
+       encode_map_3d(&mxs, dt, 2, A, K, rows, 1, lda, sa, 64, pair ? 32 : small ? 16 : 64);
   if (!ok) return TRNBLAS_ERR_ALIGN;
   ExpertsParams p{};
   if (int rc = fill_experts(p, out_dtype, rows, groups, N, K, alpha, group_sizes, sizes_64, beta, C, ldc, D, ldd))
@@ -181,7 +181,7 @@ int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t g
   if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_pair_kernel), WgradPairCfg::SMEM, pair_attr_set))
     return rc;
   static int max_pairs[64] = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = pair_config(attr, WgradPairCfg::THREADS, WgradPairCfg::SMEM, stream);
   int pairs = 0;
   if (int rc = resident_pairs(wgrad_pair_kernel, cfg, max_pairs, pairs)) return rc;

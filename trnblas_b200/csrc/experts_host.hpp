@@ -38,8 +38,8 @@ inline int smem_attribute(const void* kernel, int bytes, bool (&done)[64]) {
   return TRNBLAS_OK;
 }
 
-inline cudaLaunchConfig_t pair_config(cudaLaunchAttribute (&attr)[1], int threads, int smem,
-                                      cudaStream_t stream) {
+inline cudaLaunchConfig_t pair_config(cudaLaunchAttribute (&attr)[2], int threads, int smem,
+                                      cudaStream_t stream, bool dependent = false) {
   cudaLaunchConfig_t cfg{};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -49,8 +49,10 @@ inline cudaLaunchConfig_t pair_config(cudaLaunchAttribute (&attr)[1], int thread
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = dependent ? 2 : 1;
   return cfg;
 }
 
@@ -116,8 +118,18 @@ int launch_experts(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorM
   static bool attr_set[64] = {};
   if (int rc = smem_attribute(reinterpret_cast<const void*>(kern), Cfg::SMEM, attr_set)) return rc;
   const int grid = static_cast<int>(std::min<long long>(tiles, num_sms()));
-  kern<<<grid, Cfg::THREADS, Cfg::SMEM, stream>>>(mw, mx, mx64, msw, msx, p);
-  cudaError_t e = cudaGetLastError();
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.after_quantise ? 1 : 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaError_t e =
+      cudaLaunchKernelEx(&cfg, kern, mw, mx, mx64, msw, msx, static_cast<const ExpertsParams>(p));
   return e == cudaSuccess ? TRNBLAS_OK : cuda_fail(e, "grouped product kernel launch");
 }
 
@@ -133,8 +145,8 @@ int launch_experts_pair(const CUtensorMap& mw, const CUtensorMap& mx, const CUte
   auto kern = experts_pair_kernel<KIND, BN>;
   static bool attr_set[64] = {};
   static int max_pairs[64] = {};
-  cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = pair_config(attr, Cfg::THREADS, Cfg::SMEM, stream);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = pair_config(attr, Cfg::THREADS, Cfg::SMEM, stream, p.after_quantise != 0);
   if (int rc = smem_attribute(reinterpret_cast<const void*>(kern), Cfg::SMEM, attr_set)) return rc;
   int pairs = 0;
   if (int rc = resident_pairs(kern, cfg, max_pairs, pairs)) return rc;

@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
+  if (Cfg::MX && p.after_quantise) wait_prerequisites();
+
   const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
   const int num_tiles = tb.tile0[p.groups + 1];
   const int work_tiles = num_kb ? tb.tile0[p.groups] : 0;

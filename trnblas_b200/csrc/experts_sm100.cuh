@@ -55,7 +55,7 @@ struct ExpertsParams {
   const void* sizes;  // device, int32 or int64; nullptr: one group of all rows
   int sizes64;
   int in_fmt;   // kExpF16: kFmtBF16 / kFmtF16
-  int w_mn;     // kExpF16: weights stored K x N
+  int w_mn;     // kExpF16: weights stored K x N (2: read in boxes of 128 columns)
   int w_shared; // kExpF16: one matrix for every group
   int out_kind;
   float alpha, beta;
@@ -65,6 +65,7 @@ struct ExpertsParams {
   long long ldd;
   int tiles_w;  // weight tiles of 128
   int w_blocks;  // kExpMx4: scale blocks of one weight matrix
+  int after_quantise;  // launched beside the kernel that writes the rows
   int* status;
   unsigned long long timeout_ns;
 };
@@ -185,6 +186,7 @@ struct ExpCfg {
   static constexpr int BK = MX ? 256 : 64;  // one 128-byte swizzle row of K
   static constexpr int W_TILE = 128 * 128;
   static constexpr int X_TILE = BN * 128;
+  static constexpr int XBOX = BN == 64 ? 16 : 64;  // rows of a small box
   // rows start at a multiple of STEP in their group; with 64 a tile of 64 rows
   // lies in one scale block and one of 192 in two
   static constexpr int STEP = MX ? 64 : 16;
@@ -291,16 +293,18 @@ __device__ __forceinline__ void exp_store(const ExpertsParams& p, int r0, int le
   }
 }
 
-// map_w: the weights (kExpF16: K-major boxes of 64 K x 128 N, or MN-major of
-// 64 N x 64 K; kExpMx4: 128 bytes x 128 rows). map_x / map_x64: the rows, in
-// boxes of BN and of 64 rows (a tile of few rows loads only what it needs).
+// map_w: the weights (kExpF16: K-major boxes of 64 K x 128 N, MN-major ones of
+// 64 N x 64 K, or (p.w_mn == 2) both 64-column blocks in one box; kExpMx4: 128
+// bytes x 128 rows). map_x / map_xs: the rows, in boxes of BN and of XBOX: a
+// tile of few rows loads only what it needs. A copy takes about 80 cycles and
+// one more per 100 bytes whatever waits for it, which bounds tiles of few rows.
 // map_sw / map_sx (kExpMx4): the scales as 128 words x K blocks x row blocks,
 // in boxes of 2 K blocks and 1 / XBLK row blocks.
 template <int KIND, int BN>
 __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     experts_kernel(const __grid_constant__ CUtensorMap map_w,
                    const __grid_constant__ CUtensorMap map_x,
-                   const __grid_constant__ CUtensorMap map_x64,
+                   const __grid_constant__ CUtensorMap map_xs,
                    const __grid_constant__ CUtensorMap map_sw,
                    const __grid_constant__ CUtensorMap map_sx, const ExpertsParams p) {
   using Cfg = ExpCfg<KIND, BN>;
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     fence_barrier_init();
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
-    tma_prefetch_desc(&map_x64);
+    tma_prefetch_desc(&map_xs);
     if (Cfg::MX) {
       tma_prefetch_desc(&map_sw);
       tma_prefetch_desc(&map_sx);
@@ -356,6 +360,8 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
+  if (Cfg::MX && p.after_quantise) wait_prerequisites();
+
   const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
   const int num_tiles = tb.tile0[p.groups + 1];
   // tiles with products; the ones behind are stores of beta * C alone
@@ -369,9 +375,9 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     const bool aborted = [&] {
     for (int t = blockIdx.x; t < work_tiles; t += gridDim.x) {
       const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
-      // above three quarters of the tile one full box, else boxes of 64 rows
-      const int boxes = (BN == 64 || e.nv > BN * 3 / 4) ? 0 : (e.nv + 63) / 64;
-      const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * 64 * 128 : Cfg::X_TILE);
+      // above three quarters of the tile one full box, else small boxes
+      const int boxes = e.nv > BN * 3 / 4 ? 0 : (e.nv + Cfg::XBOX - 1) / Cfg::XBOX;
+      const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * Cfg::XBOX * 128 : Cfg::X_TILE);
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
           return true;
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
           tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, e.g);
           if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
           for (int j = 0; j < boxes; ++j)
-            tma_load_3d(sx + j * 8192, &map_x64, &full_bar[stage], k0, e.r0 + 64 * j, 0);
+            tma_load_3d(sx + j * Cfg::XBOX * 128, &map_xs, &full_bar[stage], k0, e.r0 + Cfg::XBOX * j, 0);
           uint8_t* sf = sx + Cfg::X_TILE;
           tma_load_3d(sf, &map_sw, &full_bar[stage], 0, 2 * kb, e.g * p.w_blocks + (e.n0 >> 7));
           tma_load_3d(sf + Cfg::SFW, &map_sx, &full_bar[stage], 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
@@ -393,13 +399,15 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
           const int gw = p.w_shared ? 0 : e.g;
           if (!p.w_mn) {
             tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, gw);
+          } else if (p.w_mn == 2) {
+            tma_load_4d(sw, &map_w, &full_bar[stage], 0, k0, e.n0 >> 6, gw);
           } else {
             tma_load_3d(sw, &map_w, &full_bar[stage], e.n0, k0, gw);
             tma_load_3d(sw + 8192, &map_w, &full_bar[stage], e.n0 + 64, k0, gw);
           }
           if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
           for (int j = 0; j < boxes; ++j)
-            tma_load_3d(sx + j * 8192, &map_x64, &full_bar[stage], k0, e.r0 + 64 * j, 0);
+            tma_load_3d(sx + j * Cfg::XBOX * 128, &map_xs, &full_bar[stage], k0, e.r0 + Cfg::XBOX * j, 0);
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -438,7 +446,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
       const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
       const uint32_t nm = warp_uniform(static_cast<uint32_t>((e.nv + 15) & ~15));
       const uint32_t xcol = warp_uniform(static_cast<uint32_t>(e.x0 >> 5) & 3u);  // in its scale block
-      const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn, 0, 128, nm);
+      const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn ? 1 : 0, 0, 128, nm);
       const uint32_t id2 = idesc_mx4(nm, 2);
       const int buf = tc & 1;
       if (!mbar_wait_warp(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;

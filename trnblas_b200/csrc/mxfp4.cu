@@ -158,35 +158,43 @@ __device__ __forceinline__ GroupTable block_table(int* mem, const GroupArgs& ga)
   return tb;
 }
 
-// A warp takes 4 rows 32 apart x 256 values, its lanes 8 neighbouring values of
-// a row each: 16-byte loads, four in flight, and 128-byte stores. The four
-// rows' scale words are neighbours, and the eight warps of a block hold
-// neighbouring ones, so a K block's words leave as 128 contiguous bytes.
-// Blocks walk K with stride gridDim.y. Bounded by the read of X.
+// A warp takes 4 rows x 256 values, its lanes 8 neighbouring values of a row
+// each: 16-byte loads, four in flight and the next chunk's behind them, and
+// 128-byte stores. Blocks walk K with stride gridDim.y. Bounded by the read of X.
+//
+// A stack's rows lie 32 apart in a warp: their scale words are neighbours, and
+// the eight warps of a block hold neighbouring ones, so a K block's words leave
+// as 128 contiguous bytes. Rows grouped by expert (GROUPED) are taken in their
+// own order, 32 to a block, and each word goes to its group's blocks: the first
+// loads do not wait for the scan of the sizes, and short groups make no empty
+// blocks (64 rows of 32 groups x 4096: 14 us by blocks of the groups, 5 so).
 template <typename T, bool GROUPED>
 __global__ void __launch_bounds__(256)
     mxfp4_quantize_kernel(const T* __restrict__ X, long long ldx, GroupArgs ga, int per_matrix, int K, int vec,
-                          uint8_t* __restrict__ data, long long ldq, uint4* __restrict__ scales) {
+                          uint8_t* __restrict__ data, long long ldq, uint32_t* __restrict__ scales) {
   __shared__ int mem[GROUPED ? 2 * (kMaxGroups + 2) : 1];
+  launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int blk = blockIdx.x >> 2;
-  BlockRows br;
-  if constexpr (GROUPED) {
-    const GroupTable tb = block_table(mem, ga);
-    br = group_block(tb, ga.groups, blk);
-    if (br.limit == 0) return;
-  } else {
-    br = stack_block(blk, ga.rows, per_matrix);
-  }
-  const int l32 = (blockIdx.x & 3) * 8 + warp;  // row % 32
-  const int l0 = br.local0 + l32;
   const int kwords = (K + 127) >> 7;
+  const int blk = blockIdx.x >> 2;
+  const int l32 = (blockIdx.x & 3) * 8 + warp;  // a stack's row % 32
   bool ok[4];
   long long row[4];
+  if constexpr (GROUPED) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ok[i] = l0 + 32 * i < br.limit;
-    row[i] = ok[i] ? br.base + l0 + 32 * i : br.base;
+    for (int i = 0; i < 4; ++i) {
+      const long long r = static_cast<long long>(blockIdx.x) * 32 + warp * 4 + i;
+      ok[i] = r < ga.rows;
+      row[i] = ok[i] ? r : 0;
+    }
+  } else {
+    const BlockRows br = stack_block(blk, ga.rows, per_matrix);
+    const int l0 = br.local0 + l32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ok[i] = l0 + 32 * i < br.limit;
+      row[i] = ok[i] ? br.base + l0 + 32 * i : br.base;
+    }
   }
   const int kstep = gridDim.y * 256;
   int k = blockIdx.y * 256 + lane * 8;
@@ -197,6 +205,24 @@ __global__ void __launch_bounds__(256)
       dst[i] = load8(X + row[i] * ldx + (at < K ? at : 0), ok[i] ? K - at : 0, vec);
   };
   fetch(cur, k);
+  long long word_at[4];  // GROUPED: each row's first word (K block 0), -1 behind the last group
+  if constexpr (GROUPED) {
+    const GroupTable tb = block_table(mem, ga);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = static_cast<int>(row[i]);
+      int lo = 0, hi = ga.groups;  // row0[lo] <= r
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tb.row0[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      const int l = r - tb.row0[lo];
+      word_at[i] = ok[i] && r < tb.row0[ga.groups]
+                       ? static_cast<long long>(tb.blk0[lo] + (l >> 7)) * kwords * 128 + (l & 31) * 4 + ((l >> 5) & 3)
+                       : -1;
+    }
+  }
   for (; k - lane * 8 < K; k += kstep) {
     if (k - lane * 8 + kstep < K) fetch(nxt, k + kstep);  // in flight while this chunk is converted
     uint32_t word[4];
@@ -213,9 +239,16 @@ __global__ void __launch_bounds__(256)
       word[i] = b;
     }
     const int kw = k >> 7;
-    if ((lane & 15) == 0 && kw < kwords)
-      scales[(static_cast<long long>(blk) * kwords + kw) * 32 + l32] =
-          make_uint4(word[0], word[1], word[2], word[3]);
+    if ((lane & 15) == 0 && kw < kwords) {
+      if constexpr (GROUPED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (word_at[i] >= 0) scales[word_at[i] + static_cast<long long>(kw) * 128] = word[i];
+      } else {
+        reinterpret_cast<uint4*>(scales)[(static_cast<long long>(blk) * kwords + kw) * 32 + l32] =
+            make_uint4(word[0], word[1], word[2], word[3]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
   }
@@ -385,12 +418,12 @@ unsigned k_blocks(long long xblocks, long long K) {
 }
 
 template <bool GROUPED>
-int launch_quantize(int dtype, const GroupArgs& ga, long long blocks, int per_matrix, int64_t K, const void* X,
+int launch_quantize(int dtype, const GroupArgs& ga, long long xblocks, int per_matrix, int64_t K, const void* X,
                     int64_t ldx, void* data, int64_t ldq, void* scales, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(blocks * 4), k_blocks(blocks * 4, K));
+  const dim3 grid(static_cast<unsigned>(xblocks), k_blocks(xblocks, K));
   const int vec = al16(X) && (ldx * (dtype == TRNBLAS_F32 ? 4 : 2)) % 16 == 0;
   uint8_t* q = static_cast<uint8_t*>(data);
-  uint4* s = static_cast<uint4*>(scales);
+  uint32_t* s = static_cast<uint32_t*>(scales);
   const int k = static_cast<int>(K);
   if (dtype == TRNBLAS_F32)
     mxfp4_quantize_kernel<float, GROUPED>
@@ -431,12 +464,13 @@ size_t scale_bytes(int64_t rows, int64_t groups, int64_t K) {
   return static_cast<size_t>(ceil_div(rows, 128) + groups) * ceil_div(K, 128) * 512;
 }
 
-// The product on data and scales in place; `grouped`: the rows' scales start a
-// block with every group.
+// The product on data and scales in place (with group sizes the rows' scales
+// start a block with every group). `after_quantise`: the launch before it in the
+// stream is the quantiser, which lets this kernel set up while it runs.
 int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, float alpha, const void* A,
                    int64_t lda, const void* scalesA, const void* B, int64_t ldb, const void* scalesB,
                    const void* group_sizes, int sizes_64, float beta, const void* C, int64_t ldc, void* D,
-                   int64_t ldd, cudaStream_t stream) {
+                   int64_t ldd, bool after_quantise, cudaStream_t stream) {
   const auto dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   const uint64_t kb = static_cast<uint64_t>(round_up(K, 32) / 2);
   // as for 16 bits: short row tiles and a deep pipeline where a group has at
@@ -455,7 +489,7 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   CUtensorMap mw, mx, mxs, msw, msx;
   if (!encode_map_3d(&mw, dt, 1, B, kb, N, groups, ldb, ldb * N, 128, 128) ||
       !encode_map_3d(&mx, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, small ? 64 : pair ? kMxPairBN / 2 : 192) ||
-      !encode_map_3d(&mxs, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, pair ? 32 : 64) ||
+      !encode_map_3d(&mxs, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, pair ? 32 : small ? 16 : 64) ||
       !scale_map(&msw, scalesB, wb * groups, 1) ||
       !scale_map(&msx, scalesA, ceil_div(rows, 128) + (group_sizes ? groups : 0), small ? 1 : 2))
     return TRNBLAS_ERR_ALIGN;
@@ -463,6 +497,7 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   if (int rc = fill_experts(p, out_dtype, rows, groups, N, K, alpha, group_sizes, sizes_64, beta, C, ldc, D, ldd))
     return rc;
   p.w_blocks = static_cast<int>(wb);
+  p.after_quantise = after_quantise;
   if (small) return launch_experts<kExpMx4, 64>(mw, mx, mxs, msw, msx, p, stream);
   if (pair) return launch_experts_pair<kExpMx4, kMxPairBN>(mw, mx, mxs, msw, msx, p, stream);
   return launch_experts<kExpMx4, 192>(mw, mx, mxs, msw, msx, p, stream);
@@ -482,7 +517,7 @@ int trnblas_mxfp4_quantize(int dtype, int64_t matrices, int64_t rows, int64_t K,
   GroupArgs ga{};
   ga.rows = static_cast<int>(rows);
   const int per = static_cast<int>(ceil_div(rows, 128));
-  return launch_quantize<false>(dtype, ga, matrices * per, per, K, X, ldx, data, ldq, scales,
+  return launch_quantize<false>(dtype, ga, matrices * per * 4, per, K, X, ldx, data, ldq, scales,
                                 static_cast<cudaStream_t>(stream));
 }
 
@@ -546,7 +581,7 @@ int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, i
     scalesA = workspace;
   }
   return launch_mx_gemm(out_dtype, rows, groups, N, K, alpha, A, lda, scalesA, B, ldb, scalesB, group_sizes,
-                        sizes_64, beta, C, ldc, D, ldd, stream);
+                        sizes_64, beta, C, ldc, D, ldd, false, stream);
 }
 
 size_t trnblas_mxfp4_gemm_x_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped) {
@@ -585,11 +620,11 @@ int trnblas_mxfp4_gemm_x(int a_dtype, int out_dtype, int64_t rows, int64_t group
   if (!ga.status) return TRNBLAS_ERR_CUDA;
   const int per = static_cast<int>(ceil_div(rows, 128));
   if (int rc = group_sizes
-                   ? launch_quantize<true>(a_dtype, ga, per + groups, per, K, X, ldx, data, ldq, scales, stream)
-                   : launch_quantize<false>(a_dtype, ga, per, per, K, X, ldx, data, ldq, scales, stream))
+                   ? launch_quantize<true>(a_dtype, ga, ceil_div(rows, 32), per, K, X, ldx, data, ldq, scales, stream)
+                   : launch_quantize<false>(a_dtype, ga, per * 4, per, K, X, ldx, data, ldq, scales, stream))
     return rc;
   return launch_mx_gemm(out_dtype, rows, groups, N, K, alpha, data, ldq, scales, B, ldb, scalesB, group_sizes,
-                        sizes_64, beta, C, ldc, D, ldd, stream);
+                        sizes_64, beta, C, ldc, D, ldd, true, stream);
 }
 
 }  // extern "C"
