@@ -11,8 +11,6 @@ the sm_100a kernels through the C ABI; other dtypes raise TypeError.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _native as N
@@ -23,27 +21,37 @@ DTYPES = (torch.bfloat16, torch.float16)
 MAX_GROUPS = 1024
 
 
-def _on(dev: torch.device):
-    """The operands' device current, for a call made with another one current."""
+def call_on(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) on dev's current stream, with dev the current device."""
+    stream = N.stream_ptr(dev)
     if dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+        return fn(*args, stream)
+    with torch.cuda.device(dev):
+        return fn(*args, stream)
 
 
 def _same_cuda_device(*ts) -> bool:
     """Every tensor (or None) on one CUDA device: nothing to move."""
     d = ts[0].get_device()
-    return d >= 0 and all(t is None or (isinstance(t, torch.Tensor) and t.get_device() == d) for t in ts)
+    if d < 0:
+        return False
+    for t in ts:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != d):
+            return False
+    return True
 
 
 def _check_types(name: str, a, b, out_dtype):
     for x in (a, b):
         if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES:
             raise TypeError(f"{name}: operands are bfloat16 or float16 tensors, got {getattr(x, 'dtype', type(x))}")
-    if a.dtype != b.dtype:
+    dtype = a.dtype
+    if dtype != b.dtype:
         _mixed_dtype_error(a, b)
-    out = a.dtype if out_dtype is None else out_dtype
-    if out not in (a.dtype, torch.float32):
+    if out_dtype is None:
+        return dtype
+    out = out_dtype
+    if out not in (dtype, torch.float32):
         raise TypeError(f"{name}: out_dtype is {a.dtype} or float32, got {out_dtype}")
     return out
 
@@ -63,6 +71,9 @@ def check_group_sizes(name: str, sizes, groups: int | None, rows: int) -> None:
 
 def _rows_operand(x: torch.Tensor):
     """(tensor, ld) of a rows x cols operand stored row by row on 16 bytes."""
+    s0, s1 = x.stride()
+    if s1 == 1 and s0 % 8 == 0 and s0 >= x.shape[1] and x.data_ptr() % 16 == 0 and s0:
+        return x, s0
     t, ld, tr = _tma_operand(x, x.element_size())
     if tr:
         t, ld, tr = _tma_operand(x.contiguous(), x.element_size())
@@ -105,12 +116,12 @@ def _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype):
     c_arg, ldc = _c_operand(C, Nn) if C is not None else (None, 0)
     if not sizes.is_contiguous():
         sizes = sizes.contiguous()
-    with _on(dev):
-        rc = N.lib().trnblas_grouped_gemm(
-            N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(at), lda,
-            N.ptr(bt), ldb, sb, int(tb), N.ptr(sizes), int(sizes.dtype == torch.int64),
-            float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, N.ptr(out), Nn, N.stream_ptr(dev))
-    N.check(rc, "trnblas_grouped_gemm")
+    rc = call_on(
+        dev, N.lib().trnblas_grouped_gemm, N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha),
+        at.data_ptr(), lda, bt.data_ptr(), ldb, sb, tb, sizes.data_ptr(), sizes.dtype == torch.int64,
+        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, out.data_ptr(), Nn)
+    if rc:
+        N.check(rc, "trnblas_grouped_gemm")
     N.count_launches(1)
     return out
 
@@ -131,12 +142,12 @@ def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
         sc = c_arg.stride(0)
     if not sizes.is_contiguous():
         sizes = sizes.contiguous()
-    with _on(dev):
-        rc = N.lib().trnblas_grouped_gemm_wgrad(
-            N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, M, Nn, float(alpha), N.ptr(at), lda,
-            N.ptr(bt), ldb, N.ptr(sizes), int(sizes.dtype == torch.int64),
-            float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, sc, N.ptr(out), Nn, M * Nn, N.stream_ptr(dev))
-    N.check(rc, "trnblas_grouped_gemm_wgrad")
+    rc = call_on(
+        dev, N.lib().trnblas_grouped_gemm_wgrad, N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, M, Nn, float(alpha),
+        at.data_ptr(), lda, bt.data_ptr(), ldb, sizes.data_ptr(), sizes.dtype == torch.int64,
+        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, sc, out.data_ptr(), Nn, M * Nn)
+    if rc:
+        N.check(rc, "trnblas_grouped_gemm_wgrad")
     N.count_launches(1)
     return out
 
@@ -198,15 +209,18 @@ def grouped_gemm(
     or capture forward and backward together on leaves used on no other stream.
     """
     name = "grouped_gemm"
-    transB = trans_flag(transB, "transB")
+    if transB is not False and transB is not True:
+        transB = trans_flag(transB, "transB")
     out_dtype = _check_types(name, A, B, out_dtype)
     if A.dim() != 2 or B.dim() != 3:
         raise ValueError(f"{name}: A is 2-D and B 3-D, got {tuple(A.shape)} and {tuple(B.shape)}")
     if A.shape[1] != B.shape[2 if transB else 1]:
         raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, B {tuple(B.shape)}, transB={transB}")
     check_group_sizes(name, group_sizes, B.shape[0], A.shape[0])
-    grad = torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)
-    if not grad and C is None and _same_cuda_device(A, B, group_sizes):
+    grad = (A.requires_grad or B.requires_grad) and torch.is_grad_enabled()
+    if C is None and _same_cuda_device(A, B, group_sizes):
+        if grad:
+            return _GroupedGemm.apply(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
         return _grouped(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)

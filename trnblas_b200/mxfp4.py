@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _native as N
-from .experts import _c_operand, _on, _same_cuda_device, check_group_sizes
+from .experts import _c_operand, _same_cuda_device, call_on, check_group_sizes
 from .level3 import _add_c, _cuda_device, _fuse_c, _home, _to
 
 BLOCK = 32
@@ -133,14 +133,15 @@ def _quantize(x: torch.Tensor) -> MXFP4Tensor:
     x2, ldx, rows, K = _rows2d(x)
     lead = x.shape[:-1]
     ldq = _round_up(K, BLOCK) // 2
-    data = torch.empty((*lead, ldq), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_shape(x.shape), dtype=torch.uint8, device=x.device)
+    dev = x.device
+    data = torch.empty((*lead, ldq), dtype=torch.uint8, device=dev)
+    sshape = _scale_shape(x.shape)
+    scales = torch.empty(sshape, dtype=torch.uint8, device=dev)
     if rows and K:
-        with _on(x.device):
-            rc = N.lib().trnblas_mxfp4_quantize(
-                N.dtype_code(x.dtype), scales.shape[0], x.shape[-2], K, N.ptr(x2), ldx, N.ptr(data), ldq, N.ptr(scales),
-                N.stream_ptr(x.device))
-        N.check(rc, "trnblas_mxfp4_quantize")
+        rc = call_on(dev, N.lib().trnblas_mxfp4_quantize, N.dtype_code(x.dtype), sshape[0], x.shape[-2], K,
+                     x2.data_ptr(), ldx, data.data_ptr(), ldq, scales.data_ptr())
+        if rc:
+            N.check(rc, "trnblas_mxfp4_quantize")
         N.count_launches(1)
     return _unchecked(data, scales, x.shape)
 
@@ -179,11 +180,10 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.float32) -> torc
     K = q.shape[-1]
     out = torch.empty(tuple(q.shape), dtype=dtype, device=dev)
     if out.numel():
-        with _on(dev):
-            rc = N.lib().trnblas_mxfp4_dequantize(
-                N.dtype_code(dtype), q.scales.shape[0], q.shape[-2], K, N.ptr(q.data), q.data.shape[-1], N.ptr(q.scales), N.ptr(out), K,
-                N.stream_ptr(dev))
-        N.check(rc, "trnblas_mxfp4_dequantize")
+        rc = call_on(dev, N.lib().trnblas_mxfp4_dequantize, N.dtype_code(dtype), q.scales.shape[0], q.shape[-2], K,
+                     q.data.data_ptr(), q.data.shape[-1], q.scales.data_ptr(), out.data_ptr(), K)
+        if rc:
+            N.check(rc, "trnblas_mxfp4_dequantize")
         N.count_launches(1)
     return out if home == dev else _home(out, home, dev)
 
@@ -218,32 +218,30 @@ def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
     Nn = B.shape[-2]
     G = B.shape[0] if sizes is not None else 1
     out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
-    fuse = _fuse_c(C, beta, out.shape, out_dtype, dev)
+    fuse = C is not None and _fuse_c(C, beta, out.shape, out_dtype, dev)
     if rows and Nn:
         c_arg, ldc = _c_operand(C, Nn) if fuse else (None, 0)
         if sizes is not None and not sizes.is_contiguous():
             sizes = sizes.contiguous()
-        tail = (N.ptr(B.data), B.data.shape[-1], N.ptr(B.scales), N.ptr(sizes),
-                int(sizes is not None and sizes.dtype == torch.int64), float(beta) if fuse else 0.0, N.ptr(c_arg),
-                ldc, N.ptr(out), Nn)
-        with _on(dev):
-            # scale blocks of 128 rows; with groups, a block starts with each
-            sf_bytes = (-(-rows // 128) + (G if sizes is not None else 0)) * -(-K // 128) * 512
-            if quantised:
-                ws = N.workspace(sf_bytes if sizes is not None else 0, dev)
-                rc = N.lib().trnblas_mxfp4_gemm(
-                    N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(A.data), A.data.shape[-1],
-                    N.ptr(A.scales), *tail, N.ptr(ws), sf_bytes, N.stream_ptr(dev))
-            else:
-                x, ldx, _, _ = _rows2d(A)
-                ws_bytes = rows * (_round_up(K, BLOCK) // 2) + sf_bytes
-                ws = N.workspace(ws_bytes, dev)
-                rc = N.lib().trnblas_mxfp4_gemm_x(
-                    N.dtype_code(x.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha), N.ptr(x), ldx,
-                    *tail, N.ptr(ws), ws_bytes, N.stream_ptr(dev))
-        N.check(rc, name)
+        tail = (B.data.data_ptr(), B.data.shape[-1], B.scales.data_ptr(), N.ptr(sizes),
+                sizes is not None and sizes.dtype == torch.int64, float(beta) if fuse else 0.0, N.ptr(c_arg), ldc,
+                out.data_ptr(), Nn)
+        # scale blocks of 128 rows; with groups, a block starts with each
+        sf_bytes = (-(-rows // 128) + (G if sizes is not None else 0)) * -(-K // 128) * 512
+        if quantised:
+            ws = N.workspace(sf_bytes if sizes is not None else 0, dev)
+            rc = call_on(dev, N.lib().trnblas_mxfp4_gemm, N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha),
+                         A.data.data_ptr(), A.data.shape[-1], A.scales.data_ptr(), *tail, N.ptr(ws), sf_bytes)
+        else:
+            x, ldx, _, _ = _rows2d(A)
+            ws_bytes = rows * (_round_up(K, BLOCK) // 2) + sf_bytes
+            ws = N.workspace(ws_bytes, dev)
+            rc = call_on(dev, N.lib().trnblas_mxfp4_gemm_x, N.dtype_code(x.dtype), N.dtype_code(out_dtype), rows, G, Nn,
+                         K, float(alpha), x.data_ptr(), ldx, *tail, N.ptr(ws), ws_bytes)
+        if rc:
+            N.check(rc, name)
         N.count_launches(1 if (quantised and sizes is None) or not K or not G else 2)
-    if not fuse:
+    if C is not None and not fuse:
         out = _add_c(out, beta, C.detach() if isinstance(C, torch.Tensor) else C)
     return out if home == dev else _home(out, home, dev)
 
