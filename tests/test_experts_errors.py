@@ -120,13 +120,14 @@ def test_c_entry_points_check_their_arguments():
     assert L.trnblas_mxfp4_gemm_workspace_size(300, 1, 200, 0) == 0
     assert L.trnblas_mxfp4_gemm_x_workspace_size(300, 2, 200, 1) == 300 * 112 + 5 * 2 * 512
 
-    def gx(dt=N.BF16, ws=FAKE, n=1 << 20, x=FAKE, ldx=64):
-        return L.trnblas_mxfp4_gemm_x(dt, N.BF16, 4, 1, 8, 64, 1.0, x, ldx, FAKE, 32, FAKE, None, 0, 0.0, None, 0, FAKE, 8,
+    def gx(dt=N.BF16, ws=FAKE, n=1 << 20, x=FAKE, ldx=64, rows=40):
+        return L.trnblas_mxfp4_gemm_x(dt, N.BF16, rows, 1, 8, 64, 1.0, x, ldx, FAKE, 32, FAKE, None, 0, 0.0, None, 0, FAKE, 8,
                                       ws, n, None)
 
-    for bad in (dict(dt=N.F64), dict(x=None), dict(ldx=63)):
+    assert L.trnblas_mxfp4_gemm_x_workspace_size(16, 1, 1 << 14, 0) == 0  # a few rows quantise in the product
+    for bad in (dict(dt=N.F64), dict(x=None), dict(ldx=63), dict(rows=4, x=None), dict(rows=4, ldx=63)):
         assert gx(**bad) == N.ERR_ARG, bad
-    for bad in (dict(ws=None), dict(ws=FAKE + 8), dict(n=4 * 32 + 511)):
+    for bad in (dict(ws=None), dict(ws=FAKE + 8), dict(n=40 * 32 + 511)):
         assert gx(**bad) == N.ERR_WORKSPACE, bad
 
 

@@ -134,11 +134,46 @@ def test_whole_numbers_are_exact():
 def test_operand_quantised_on_the_way(dt, M):
     x, qb = _rand(M, 200, dt=dt), tb.quantize_mxfp4(_rand(72, 200, seed=3))
     D = tb.gemm_mxfp4(1.0, x, qb)
-    assert torch.equal(D, tb.gemm_mxfp4(1.0, tb.quantize_mxfp4(x), qb))
+    if M > 16:  # (a few rows split K over CTAs: another order of the same sum)
+        assert torch.equal(D, tb.gemm_mxfp4(1.0, tb.quantize_mxfp4(x), qb))
     a = X.dequantize(*X.quantize(x), 200)
     b = _values(qb)
     ref = a @ b.T
     X.check(D, ref, X.tolerance(ref, a.abs() @ b.abs().T, 200, BF))
+
+
+@pytest.mark.parametrize("M", [1, 2, 7, 16])
+@pytest.mark.parametrize("Nn,K", [(8, 32), (128, 256), (130, 1000), (520, 4096), (200, 33), (64, 8200), (2048, 700),
+                                  (136, 45056), (64, 44000), (128, 50000)])
+def test_few_rows(M, Nn, K):
+    """Rows quantised inside the product, K split over a cluster: as many
+    splits as fit, blocks that end inside a rank's share, and ranks with none."""
+    dt = (BF, FP, F32)[M % 3]
+    x, qb = _rand(M, K, dt=dt), _rand_mx(Nn, K, seed=3)
+    a, b = X.dequantize(*X.quantize(x), K), _values(qb)
+    ref, mags = a @ b.T, a.abs() @ b.abs().T
+    C = _rand(M, Nn, dt=F32)
+    X.check(tb.gemm_mxfp4(1.0, x, qb), ref, X.tolerance(ref, mags, K, BF))
+    ref2 = 0.5 * ref - 2.0 * C.double()
+    D = tb.gemm_mxfp4(0.5, x, qb, -2.0, C, out_dtype=F32)
+    X.check(D, ref2, X.tolerance(ref2, mags, K, F32, 2.0 * C))
+    assert torch.equal(D, tb.gemm_mxfp4(0.5, x, qb, -2.0, C, out_dtype=F32))
+    big = torch.zeros(M, 2 * K + 8, dtype=dt, device=DEV)  # rows off 16 bytes and far apart
+    big[:, 1:K + 1] = x
+    assert torch.equal(tb.gemm_mxfp4(1.0, big[:, 1:K + 1], qb), tb.gemm_mxfp4(1.0, x, qb))
+    assert tb.device_status(0) == 0
+
+
+def test_few_rows_with_nan_and_infinity():
+    x, qb = _rand(5, 600), tb.quantize_mxfp4(_rand(72, 600))
+    clean = tb.gemm_mxfp4(1.0, x, qb)
+    x[1, 599], x[3, 0] = float("inf"), float("nan")
+    D = tb.gemm_mxfp4(1.0, x, qb)
+    assert torch.equal(D[[0, 2, 4]], clean[[0, 2, 4]]) and D[[1, 3]].isnan().all()
+    s = torch.randint(100, 140, (72, 19), dtype=torch.uint8, device=DEV, generator=_gen(2))
+    s[11, 18] = 255  # a NaN block among the weights
+    D = tb.gemm_mxfp4(1.0, x[:1], tb.MXFP4Tensor.from_parts(qb.parts()[0], s, 600))
+    assert D[0, 11].isnan() and D.isnan().sum() == 1
 
 
 def test_alpha_beta_c_and_nan_scales():

@@ -12,114 +12,11 @@
 #include <algorithm>
 
 #include "experts_host.hpp"
+#include "mxfp4_convert.cuh"
+#include "mxfp4_token_sm100.cuh"
 
 namespace tb {
 namespace {
-
-// Eight neighbouring values of a row as they are stored.
-template <typename T>
-struct Raw8 {
-  uint4 v[sizeof(T) / 2];
-};
-
-template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* src, int valid, bool vec) {
-  Raw8<T> r;
-  constexpr int V = static_cast<int>(sizeof(T)) / 2;
-  if (vec && valid >= 8) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-    return r;
-  }
-  uint32_t w[4 * V] = {};
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < valid) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < valid)
-        w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(src) + i)) << (16 * (i & 1));
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  return r;
-}
-
-// 8 E2M1 codes of 8 floats, the first in the lowest bits: nearest, ties to
-// even, saturating at 6.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&u)[8]) {
-  uint32_t w;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(w)
-      : "f"(u[0]), "f"(u[1]), "f"(u[2]), "f"(u[3]), "f"(u[4]), "f"(u[5]), "f"(u[6]), "f"(u[7]));
-  return w;
-}
-
-// Four lanes hold a block of 32 (8 values each). The block's unit is 2^(s - 127)
-// with s = max(E, 2) - 2, E the biased fp32 exponent of the block's largest
-// magnitude: the largest power of two not above it, divided by 4 (E2M1's
-// largest power of two). Scaling by it is exact; the conversion rounds to the
-// nearest of 0, .5, 1, 1.5, 2, 3, 4, 6, ties to even, and saturates (a block's
-// largest magnitude is below 8 units). A block that holds an infinity or a NaN
-// gets the NaN scale 255. The maximum is taken on the magnitudes' bits, which
-// order as the values do (16-bit types: two at a time).
-template <typename T>
-__device__ __forceinline__ uint32_t quantize8(const Raw8<T>& r, uint32_t& s) {
-  float x[8];
-  uint32_t E;
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t w[8] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w, r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = max(m, w[i] & 0x7FFFFFFFu);
-      x[i] = __uint_as_float(w[i]);
-    }
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    E = m >> 23;
-  } else {
-    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-    uint32_t m = __vimax3_u16x2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu, w[2] & 0x7FFF7FFFu);
-    uint32_t o = __shfl_xor_sync(0xffffffffu, m = __vimax3_u16x2(m, w[3] & 0x7FFF7FFFu, 0u), 1);
-    m = __vimax3_u16x2(m, o, 0u);
-    o = __shfl_xor_sync(0xffffffffu, m, 2);
-    m = __vimax3_u16x2(m, o, 0u);
-    m = max(m & 0xFFFFu, m >> 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-      }
-    }
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      E = m >> 7;
-    else
-      E = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m)))) >> 23;
-  }
-  s = max(E, 2u) - 2u;
-  const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s), normal
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= inv;
-  uint32_t w = e2m1x8(x);
-  if (E == 255) {
-    s = 255;
-    w = 0;
-  }
-  return w;
-}
 
 // Which rows a scale block holds: local rows 0 .. limit - 1 at `base` + local.
 struct BlockRows {
@@ -464,6 +361,72 @@ size_t scale_bytes(int64_t rows, int64_t groups, int64_t K) {
   return static_cast<size_t>(ceil_div(rows, 128) + groups) * ceil_div(K, 128) * 512;
 }
 
+// A few rows of a dense product go to the kernel that quantises them itself.
+bool token_path(int64_t rows, int64_t K, bool grouped) {
+  return !grouped && rows <= TokenCfg::ROWS && ceil_div(K, 256) <= TokenCfg::MAX_KB * TokenCfg::MAX_SPLIT;
+}
+
+int launch_token(int a_dtype, int out_dtype, int64_t rows, int64_t N, int64_t K, float alpha, const void* X,
+                 int64_t ldx, const void* B, int64_t ldb, const void* scalesB, float beta, const void* C,
+                 int64_t ldc, void* D, int64_t ldd, cudaStream_t stream) {
+  using Cfg = TokenCfg;
+  const int64_t kw = ceil_div(K, 128), kb = ceil_div(K, 256), tiles = ceil_div(N, 128);
+  CUtensorMap mw, msw;
+  const uint64_t dims[3] = {128, static_cast<uint64_t>(kw), static_cast<uint64_t>(tiles)};
+  const uint64_t strides[2] = {128, 128 * static_cast<uint64_t>(kw)};
+  const uint32_t box[3] = {128, 2, 1};
+  if (!encode_map_3d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B, round_up(K, 32) / 2, N, 1, ldb, ldb * N, 128, 128) ||
+      !encode_map(&msw, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, scalesB, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE))
+    return TRNBLAS_ERR_ALIGN;
+  // K over enough CTAs to occupy the SMs once, at least two blocks of it each,
+  // and at most what a CTA holds
+  int split = 1;
+  while (split < Cfg::MAX_SPLIT &&
+         (ceil_div(kb, split) > Cfg::MAX_KB || (tiles * split * 2 <= num_sms() && kb >= 4 * split)))
+    split *= 2;
+  TokenParams p{};
+  p.X = X;
+  p.ldx = ldx;
+  p.vec = al16(X) && (ldx * (a_dtype == TRNBLAS_F32 ? 4 : 2)) % 16 == 0;
+  p.rows = static_cast<int>(rows);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.kb_per_cta = static_cast<int>(ceil_div(kb, split));
+  p.alpha = alpha;
+  p.beta = beta;
+  p.out_kind = out_kind_of(out_dtype);
+  p.C = C;
+  p.ldc = ldc;
+  p.D = D;
+  p.ldd = ldd;
+  p.status = status_word();
+  if (!p.status) return TRNBLAS_ERR_CUDA;
+  p.timeout_ns = wait_timeout_ns();
+  const int smem = Cfg::smem(p.kb_per_cta, split);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), 1, 1);
+  cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto launch = [&](auto kern, bool (&done)[64]) {
+    if (int rc = smem_attribute(reinterpret_cast<const void*>(kern), Cfg::smem(Cfg::MAX_KB, Cfg::MAX_SPLIT), done))
+      return rc;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, msw, static_cast<const TokenParams>(p));
+    return e == cudaSuccess ? static_cast<int>(TRNBLAS_OK) : cuda_fail(e, "mxfp4 token kernel launch");
+  };
+  static bool done[3][64] = {};
+  if (a_dtype == TRNBLAS_F32) return launch(mxfp4_token_kernel<float>, done[0]);
+  if (a_dtype == TRNBLAS_BF16) return launch(mxfp4_token_kernel<__nv_bfloat16>, done[1]);
+  return launch(mxfp4_token_kernel<__half>, done[2]);
+}
+
 // The product on data and scales in place (with group sizes the rows' scales
 // start a block with every group). `after_quantise`: the launch before it in the
 // stream is the quantiser, which lets this kernel set up while it runs.
@@ -585,7 +548,7 @@ int trnblas_mxfp4_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, i
 }
 
 size_t trnblas_mxfp4_gemm_x_workspace_size(int64_t rows, int64_t groups, int64_t K, int grouped) {
-  if (rows <= 0 || groups <= 0 || K <= 0) return 0;
+  if (rows <= 0 || groups <= 0 || K <= 0 || token_path(rows, K, grouped)) return 0;
   // packed values, then the scale blocks
   return static_cast<size_t>(rows) * (round_up(K, 32) / 2) + scale_bytes(rows, grouped ? groups : 0, K);
 }
@@ -607,6 +570,17 @@ int trnblas_mxfp4_gemm_x(int a_dtype, int out_dtype, int64_t rows, int64_t group
   if (rows == 0 || N == 0 || K == 0 || groups == 0)
     return trnblas_mxfp4_gemm(out_dtype, rows, groups, N, K, alpha, X, ldq, X, B, ldb, scalesB, group_sizes, sizes_64,
                               beta, C, ldc, D, ldd, workspace, workspace_bytes, stream_);
+  if (token_path(rows, K, group_sizes != nullptr)) {
+    // (the checks on A's pointers: X stands for them)
+    if (!X || ldx < K) {
+      set_error("trnblas_mxfp4_gemm_x: NULL X, or ldx smaller than K");
+      return TRNBLAS_ERR_ARG;
+    }
+    if (int rc = check_mx_gemm(out_dtype, rows, groups, N, K, B, ldq, scalesB, B, ldb, scalesB, group_sizes, beta, C,
+                               ldc, D, ldd))
+      return rc;
+    return launch_token(a_dtype, out_dtype, rows, N, K, alpha, X, ldx, B, ldb, scalesB, beta, C, ldc, D, ldd, stream);
+  }
   const size_t need = trnblas_mxfp4_gemm_x_workspace_size(rows, groups, K, group_sizes != nullptr);
   if (!workspace || !al16(workspace) || workspace_bytes < need) {
     set_error("trnblas_mxfp4_gemm_x: needs " + std::to_string(need) + " workspace bytes, 16-byte aligned");

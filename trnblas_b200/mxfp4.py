@@ -226,21 +226,24 @@ def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
         tail = (B.data.data_ptr(), B.data.shape[-1], B.scales.data_ptr(), N.ptr(sizes),
                 sizes is not None and sizes.dtype == torch.int64, float(beta) if fuse else 0.0, N.ptr(c_arg), ldc,
                 out.data_ptr(), Nn)
-        # scale blocks of 128 rows; with groups, a block starts with each
-        sf_bytes = (-(-rows // 128) + (G if sizes is not None else 0)) * -(-K // 128) * 512
+        ws = None
         if quantised:
-            ws = N.workspace(sf_bytes if sizes is not None else 0, dev)
+            ws_bytes = 0
+            if sizes is not None:
+                ws_bytes = N.lib().trnblas_mxfp4_gemm_workspace_size(rows, G, K, True)
+                ws = N.workspace(ws_bytes, dev)
             rc = call_on(dev, N.lib().trnblas_mxfp4_gemm, N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha),
-                         A.data.data_ptr(), A.data.shape[-1], A.scales.data_ptr(), *tail, N.ptr(ws), sf_bytes)
+                         A.data.data_ptr(), A.data.shape[-1], A.scales.data_ptr(), *tail, N.ptr(ws), ws_bytes)
         else:
             x, ldx, _, _ = _rows2d(A)
-            ws_bytes = rows * (_round_up(K, BLOCK) // 2) + sf_bytes
+            ws_bytes = N.lib().trnblas_mxfp4_gemm_x_workspace_size(rows, G, K, sizes is not None)
             ws = N.workspace(ws_bytes, dev)
             rc = call_on(dev, N.lib().trnblas_mxfp4_gemm_x, N.dtype_code(x.dtype), N.dtype_code(out_dtype), rows, G, Nn,
                          K, float(alpha), x.data_ptr(), ldx, *tail, N.ptr(ws), ws_bytes)
         if rc:
             N.check(rc, name)
-        N.count_launches(1 if (quantised and sizes is None) or not K or not G else 2)
+        # (quantiser or regrouping +) the product; a few rows quantise in the product
+        N.count_launches(2 if ws is not None else 1)
     if C is not None and not fuse:
         out = _add_c(out, beta, C.detach() if isinstance(C, torch.Tensor) else C)
     return out if home == dev else _home(out, home, dev)
