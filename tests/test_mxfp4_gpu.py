@@ -108,7 +108,8 @@ def test_quantise_layouts():
 
 
 DENSE = [(1, 128, 64), (1, 8, 32), (3, 130, 33), (17, 257, 256), (64, 128, 1000), (65, 384, 128), (200, 100, 520),
-         (192, 256, 256), (385, 200, 4096), (1000, 640, 776), (448, 129, 288), (321, 300, 640)]
+         (192, 256, 256), (385, 200, 4096), (1000, 640, 776), (448, 129, 288), (321, 300, 640),
+         (777, 4096, 520), (500, 9000, 264)]
 
 
 @pytest.mark.parametrize("M,Nn,K", DENSE)

@@ -89,7 +89,7 @@ int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups,
   p.w_shared = shared;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (small) return launch_experts<kExpF16, 64>(mw, mx, mxs, mw, mw, p, st);
-  if (pair) return launch_experts_pair<kExpF16, 256>(mw, mx, mxs, mw, mw, p, st);
+  if (pair) return launch_experts_pair<kExpF16, 256, 2>(mw, mx, mxs, mw, mw, p, st);
   return launch_experts<kExpF16, 256>(mw, mx, mxs, mw, mw, p, st);
 }
 

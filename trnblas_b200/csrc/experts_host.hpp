@@ -135,14 +135,14 @@ int launch_experts(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorM
 
 // Clusters of two CTAs, as many as can be resident at once (a cluster's CTAs
 // wait for one another only).
-template <int KIND, int BN>
+template <int KIND, int BN, int NBUF>
 int launch_experts_pair(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorMap& mx32,
                         const CUtensorMap& msw, const CUtensorMap& msx, ExpertsParams& p,
                         cudaStream_t stream) {
-  using Cfg = ExpPairCfg<KIND, BN>;
+  using Cfg = ExpPairCfg<KIND, BN, NBUF>;
   const long long tiles = bound_tiles(p, BN, 256);
   if (!tiles) return TRNBLAS_ERR_ARG;
-  auto kern = experts_pair_kernel<KIND, BN>;
+  auto kern = experts_pair_kernel<KIND, BN, NBUF>;
   static bool attr_set[64] = {};
   static int max_pairs[64] = {};
   cudaLaunchAttribute attr[2];

@@ -19,28 +19,35 @@
 
 namespace tb {
 
-template <int KIND, int BN>
+// NBUF accumulators: two, so that the next tile's MMAs run beside an epilogue,
+// or one, where a pair has one tile anyway.
+template <int KIND, int BN, int NBUF>
 struct ExpPairCfg {
   static constexpr bool MX = KIND == kExpMx4;
   static constexpr int BK = MX ? 256 : 64;
   static constexpr int HN = BN / 2;  // rows of a CTA
   static constexpr int W_TILE = 128 * 128;
   static constexpr int X_TILE = HN * 128;
-  static constexpr int STEP = MX ? 64 : 32;
+  // rows start at a multiple of STEP in their group, so that their scales lie in
+  // two blocks
+  static constexpr int STEP = !MX ? 32 : BN == 192 ? 64 : 128;
   static constexpr int XBLK = (BN + 127) / 128;
-  static_assert(!MX || BN == 192, "a tile's rows lie in two scale blocks");
+  static_assert(!MX || BN == 192 || BN == 256, "a tile's rows lie in two scale blocks");
   static constexpr int SFW = MX ? 2 * 512 : 0;
   static constexpr int SFX = MX ? 2 * XBLK * 512 : 0;
   static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
   static_assert(STAGE_BYTES % 1024 == 0 && BN % 32 == 0 && BN <= 256, "tile geometry");
-  static constexpr int FIT = (227 * 1024 - 1024 - 512 - kEpiStageBytes - kGroupTableBytes) / STAGE_BYTES;
+  // 4-bit tiles pass in half the time: two epilogue warps a TMEM lane quarter
+  static constexpr int EPI_WARPS = MX ? 8 : 4;
+  static constexpr int EPI_BYTES = EPI_WARPS * (kEpiStageBytes / 4);
+  static constexpr int FIT = (227 * 1024 - 1024 - 512 - EPI_BYTES - kGroupTableBytes) / STAGE_BYTES;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SF_COLS = MX ? 2 * 4 * (1 + XBLK) : 0;
-  static constexpr int NSLOT_FIT = MX ? (512 - 2 * BN) / (SF_COLS ? SF_COLS : 1) : 0;
+  static constexpr int NSLOT_FIT = MX ? (512 - NBUF * BN) / (SF_COLS ? SF_COLS : 1) : 0;
   static constexpr int NSLOT = NSLOT_FIT < STAGES ? NSLOT_FIT : STAGES;
   static_assert(!MX || NSLOT >= 2, "two scale slots");
-  static constexpr int THREADS = 32 * 6;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + kEpiStageBytes + kGroupTableBytes;
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + EPI_BYTES + kGroupTableBytes;
 };
 
 __device__ __forceinline__ void mma_mx4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
@@ -62,14 +69,14 @@ __device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t sde
 // map_w: as for the one-CTA kernel, or (p.w_mn == 2) MN-major in boxes of 64 N
 // x 64 K x 2 blocks of 64 N, one copy instead of two. map_x / map_x32: the
 // rows in boxes of HN and of 32.
-template <int KIND, int BN>
-__global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
+template <int KIND, int BN, int NBUF>
+__global__ void __launch_bounds__(ExpPairCfg<KIND, BN, NBUF>::THREADS, 1)
     experts_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                         const __grid_constant__ CUtensorMap map_x,
                         const __grid_constant__ CUtensorMap map_x32,
                         const __grid_constant__ CUtensorMap map_sw,
                         const __grid_constant__ CUtensorMap map_sx, const ExpertsParams p) {
-  using Cfg = ExpPairCfg<KIND, BN>;
+  using Cfg = ExpPairCfg<KIND, BN, NBUF>;
   constexpr int STAGES = Cfg::STAGES;
   constexpr uint32_t SB = Cfg::STAGE_BYTES;
 
@@ -85,7 +92,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* epi = smem + STAGES * SB + 512;
   GroupTable tb;
-  tb.row0 = reinterpret_cast<int*>(epi + kEpiStageBytes);
+  tb.row0 = reinterpret_cast<int*>(epi + Cfg::EPI_BYTES);
   tb.tile0 = tb.row0 + kMaxGroups + 2;
   tb.blk0 = Cfg::MX ? tb.tile0 + kMaxGroups + 2 : nullptr;
 
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&accf_bar[a], 1);
-      mbar_init(&acce_bar[a], 8);
+      mbar_init(&acce_bar[a], 2 * Cfg::EPI_WARPS);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -225,8 +232,8 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
       const uint32_t id = Cfg::MX ? idesc_mx4(nm, 0) + (1u << 27)  // M = 256
                                   : idesc(kAccF32, p.in_fmt, p.in_fmt, p.w_mn ? 1 : 0, 0, 256, nm);
       const uint32_t id2 = idesc_mx4(nm, 2) + (1u << 27);
-      const int buf = tc & 1;
-      if (!mbar_wait_warp(&acce_bar[buf], ((tc >> 1) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
+      const int buf = tc % NBUF;
+      if (!mbar_wait_warp(&acce_bar[buf], ((tc / NBUF) & 1) ^ 1u, ab, kTimeoutAccEmpty)) break;
       tc_fence_after();
       const uint32_t d = tmem_base + buf * BN;
       // the slot's last reader: the K block NSLOT back, its stage and phase
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
           tc_fence_after();
           const uint32_t off = s * SB;
           if constexpr (Cfg::MX) {
-            const uint32_t sfw = tmem_base + 2 * BN + (RING ? slot : s) * Cfg::SF_COLS;
+            const uint32_t sfw = tmem_base + NBUF * BN + (RING ? slot : s) * Cfg::SF_COLS;
             const uint32_t sfx = sfw + 8;
             if (++slot == Cfg::NSLOT) slot = 0;
 #pragma unroll
@@ -305,9 +312,11 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= 2 && warp < 6) {
+  } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
+    // with eight warps, chunks of 32 rows alternate between two
+    const int c0 = 32 * ((warp - 2) >> 2), cstep = 8 * Cfg::EPI_WARPS;
     void* tsm = epi + (warp - 2) * (kEpiStageBytes / 4);
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     const uint32_t acce_leader = mapa_shared(smem_u32(acce_bar), 0);
@@ -320,15 +329,15 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN>::THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) z[j] = 0.0f;
         if (n0 < p.N)
-          for (int c = 0; c < e.nv; c += 32) exp_store(p, e.r0 + c, min(32, e.nv - c), n0, z, tsm);
+          for (int c = c0; c < e.nv; c += cstep) exp_store(p, e.r0 + c, min(32, e.nv - c), n0, z, tsm);
         continue;
       }
-      const int buf = tc & 1;
-      if (!mbar_wait_warp(&accf_bar[buf], (tc >> 1) & 1, ab, kTimeoutAccFull)) break;
+      const int buf = tc % NBUF;
+      if (!mbar_wait_warp(&accf_bar[buf], (tc / NBUF) & 1, ab, kTimeoutAccFull)) break;
       ++tc;
       tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < e.nv; c += 32) {
+      for (int c = c0; c < e.nv; c += cstep) {
         uint32_t v[32];
         tmem_ld32(lane_base + buf * BN + c, v);
         tmem_ld_wait();

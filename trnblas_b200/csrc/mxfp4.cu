@@ -268,11 +268,6 @@ int check_mx(const char* what, int64_t rows, int64_t K, int64_t ldq) {
   return TRNBLAS_OK;
 }
 
-// Rows of a CTA pair's tile: two accumulators of 192 columns and the scales of
-// five stages fill TMEM.
-constexpr int kMxPairBN = 192;
-
-
 int check_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_t K, const void* A, int64_t lda,
                   const void* scalesA, const void* B, int64_t ldb, const void* scalesB, const void* group_sizes,
                   float beta, const void* C, int64_t ldc, const void* D, int64_t ldd) {
@@ -440,6 +435,13 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   // most 64 rows on average, CTA pairs above
   const bool small = rows <= 64 * groups;
   const bool pair = !small && N > 128;
+  // Pair tiles of 192 rows: two accumulators and the scales of five stages fill
+  // TMEM. Where those need a second wave of pairs and tiles of 256 with one
+  // accumulator do not, take these (dense: 777 rows x 4096 x 4010, 80 tiles of
+  // 192 against 64 of 256 on 74 pairs, see the kernel's figures).
+  const int64_t wt = ceil_div(N, 256), pairs = num_sms() / 2;
+  const bool one_wave = pair && !group_sizes && ceil_div(rows, 192) * wt > pairs && ceil_div(rows, 256) * wt <= pairs;
+  const uint32_t xbox = small ? 64 : !pair ? 192 : one_wave ? 128 : 96;
   const uint64_t kw = static_cast<uint64_t>(ceil_div(K, 128));
   const uint64_t wb = static_cast<uint64_t>(ceil_div(N, 128));
   auto scale_map = [&](CUtensorMap* m, const void* base, uint64_t blocks, uint32_t box_blocks) {
@@ -451,7 +453,7 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   };
   CUtensorMap mw, mx, mxs, msw, msx;
   if (!encode_map_3d(&mw, dt, 1, B, kb, N, groups, ldb, ldb * N, 128, 128) ||
-      !encode_map_3d(&mx, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, small ? 64 : pair ? kMxPairBN / 2 : 192) ||
+      !encode_map_3d(&mx, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, xbox) ||
       !encode_map_3d(&mxs, dt, 1, A, kb, rows, 1, lda, lda * rows, 128, pair ? 32 : small ? 16 : 64) ||
       !scale_map(&msw, scalesB, wb * groups, 1) ||
       !scale_map(&msx, scalesA, ceil_div(rows, 128) + (group_sizes ? groups : 0), small ? 1 : 2))
@@ -462,7 +464,8 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   p.w_blocks = static_cast<int>(wb);
   p.after_quantise = after_quantise;
   if (small) return launch_experts<kExpMx4, 64>(mw, mx, mxs, msw, msx, p, stream);
-  if (pair) return launch_experts_pair<kExpMx4, kMxPairBN>(mw, mx, mxs, msw, msx, p, stream);
+  if (one_wave) return launch_experts_pair<kExpMx4, 256, 1>(mw, mx, mxs, msw, msx, p, stream);
+  if (pair) return launch_experts_pair<kExpMx4, 192, 2>(mw, mx, mxs, msw, msx, p, stream);
   return launch_experts<kExpMx4, 192>(mw, mx, mxs, msw, msx, p, stream);
 }
 

@@ -30,6 +30,12 @@ def call_on(dev: torch.device, fn, *args) -> int:
         return fn(*args, stream)
 
 
+def empty(shape, dtype, dev) -> torch.Tensor:
+    """torch.empty for a 1-D or 2-D shape, by the entry that takes strides (half
+    the host time of torch.empty's parsing)."""
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=dev)
+
+
 def _same_cuda_device(*ts) -> bool:
     """Every tensor (or None) on one CUDA device: nothing to move."""
     d = ts[0].get_device()
@@ -106,7 +112,7 @@ def _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype):
     G = B.shape[0]
     Nn = B.shape[1] if transB else B.shape[2]
     dev = a.device
-    out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
+    out = empty((rows, Nn), out_dtype, dev)
     if rows == 0 or Nn == 0:
         return out
     at, lda, bt, ldb, tb, sb = a, K, B, Nn, False, 0
@@ -132,7 +138,7 @@ def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
     Nn = b.shape[1]
     G = sizes.shape[0]
     dev = a.device
-    out = torch.empty((G, M, Nn), dtype=out_dtype, device=dev)
+    out = torch.empty_strided((G, M, Nn), (M * Nn, Nn, 1), dtype=out_dtype, device=dev)
     if out.numel() == 0:
         return out
     (at, lda), (bt, ldb) = (_rows_operand(a), _rows_operand(b)) if rows else ((a, M), (b, Nn))
@@ -204,7 +210,8 @@ def grouped_gemm(
     dtype are fused; another C is added afterwards with torch semantics.
 
     Differentiable in A, B and C (once): the gradients run on the same kernels,
-    rounded once to their operand's dtype. Inside a CUDA graph capture, call
+    rounded once to their operand's dtype; an incoming float32 gradient is
+    rounded to the operands' dtype first. Inside a CUDA graph capture, call
     `grouped_gemm` (transB flipped) and `grouped_gemm_wgrad` for them directly,
     or capture forward and backward together on leaves used on no other stream.
     """

@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _native as N
-from .experts import _c_operand, _same_cuda_device, call_on, check_group_sizes
+from .experts import _c_operand, _same_cuda_device, call_on, check_group_sizes, empty
 from .level3 import _add_c, _cuda_device, _fuse_c, _home, _to
 
 BLOCK = 32
@@ -134,9 +134,12 @@ def _quantize(x: torch.Tensor) -> MXFP4Tensor:
     lead = x.shape[:-1]
     ldq = _round_up(K, BLOCK) // 2
     dev = x.device
-    data = torch.empty((*lead, ldq), dtype=torch.uint8, device=dev)
+    data = empty((rows, ldq), torch.uint8, dev)
+    if x.dim() != 2:
+        data = data.view(*lead, ldq)
     sshape = _scale_shape(x.shape)
-    scales = torch.empty(sshape, dtype=torch.uint8, device=dev)
+    _, rb, kw, _ = sshape
+    scales = torch.empty_strided(sshape, (rb * kw * 512, kw * 512, 512, 1), dtype=torch.uint8, device=dev)
     if rows and K:
         rc = call_on(dev, N.lib().trnblas_mxfp4_quantize, N.dtype_code(x.dtype), sshape[0], x.shape[-2], K,
                      x2.data_ptr(), ldx, data.data_ptr(), ldq, scales.data_ptr())
@@ -178,7 +181,8 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.float32) -> torc
         dev = _cuda_device(q.data)
         q = q.to(dev)
     K = q.shape[-1]
-    out = torch.empty(tuple(q.shape), dtype=dtype, device=dev)
+    shape = q.shape
+    out = empty(shape, dtype, dev) if len(shape) == 2 else torch.empty(tuple(shape), dtype=dtype, device=dev)
     if out.numel():
         rc = call_on(dev, N.lib().trnblas_mxfp4_dequantize, N.dtype_code(dtype), q.scales.shape[0], q.shape[-2], K,
                      q.data.data_ptr(), q.data.shape[-1], q.scales.data_ptr(), out.data_ptr(), K)
@@ -217,7 +221,7 @@ def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
     rows, K = A.shape
     Nn = B.shape[-2]
     G = B.shape[0] if sizes is not None else 1
-    out = torch.empty((rows, Nn), dtype=out_dtype, device=dev)
+    out = empty((rows, Nn), out_dtype, dev)
     fuse = C is not None and _fuse_c(C, beta, out.shape, out_dtype, dev)
     if rows and Nn:
         c_arg, ldc = _c_operand(C, Nn) if fuse else (None, 0)
@@ -231,13 +235,13 @@ def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
             ws_bytes = 0
             if sizes is not None:
                 ws_bytes = N.lib().trnblas_mxfp4_gemm_workspace_size(rows, G, K, True)
-                ws = N.workspace(ws_bytes, dev)
+                ws = empty((ws_bytes,), torch.uint8, dev) if ws_bytes else None
             rc = call_on(dev, N.lib().trnblas_mxfp4_gemm, N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha),
                          A.data.data_ptr(), A.data.shape[-1], A.scales.data_ptr(), *tail, N.ptr(ws), ws_bytes)
         else:
             x, ldx, _, _ = _rows2d(A)
             ws_bytes = N.lib().trnblas_mxfp4_gemm_x_workspace_size(rows, G, K, sizes is not None)
-            ws = N.workspace(ws_bytes, dev)
+            ws = empty((ws_bytes,), torch.uint8, dev) if ws_bytes else None
             rc = call_on(dev, N.lib().trnblas_mxfp4_gemm_x, N.dtype_code(x.dtype), N.dtype_code(out_dtype), rows, G, Nn,
                          K, float(alpha), x.data_ptr(), ldx, *tail, N.ptr(ws), ws_bytes)
         if rc:

@@ -17,6 +17,11 @@ outputs are fresh.
     ozaki_gemm(a, b, k) -> float64                fp64-class a @ b on the int8 pipe
     pair_energy(B, eo, ev, p0, p1) -> float64 0-d the pair-range DF-MP2 energy
 
+    grouped_gemm(a, b, group_sizes, alpha, tb, out_dtype)       rows by expert (with autograd)
+    grouped_gemm_wgrad(a, b, group_sizes, alpha, out_dtype)     its weights' gradient
+    quantize_mxfp4(x) -> (data, scales)           and dequantize_mxfp4(data, scales, k, dtype)
+    gemm_mxfp4(x, b_data, b_scales, alpha, out_dtype)           and grouped_gemm_mxfp4 (+ group_sizes)
+
 `OPS[name](*args)` calls the op after the reference's operand dtype check:
 a tensor of a dtype the kernel does not take raises TypeError naming the op.
 """
@@ -26,7 +31,9 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from . import experts as _ex
 from . import level3 as _l3
+from . import mxfp4 as _mx
 
 _F16 = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -207,3 +214,107 @@ OPS = {name: _dtype_checked(name, op) for name, op in _RAW.items()}
 
 __all__ = ["OPS", "KERNEL_DTYPES", "check_kernel_operands", "gemm", "batched_gemm", "syrk",
            "ozaki_split", "ozaki_gemm", "pair_energy"]
+
+
+# ── products grouped by expert and in 4 bits ────────────────────────────────
+# No counterparts in the reference, so they stand in a table of their own.
+# The 4-bit operands are the (data, scales) pairs of `MXFP4Tensor`; `rows` and
+# `k` are its logical sizes.
+
+
+@torch.library.custom_op("trnblas::grouped_gemm", mutates_args=(), device_types="cuda")
+def grouped_gemm(a: torch.Tensor, b: torch.Tensor, group_sizes: torch.Tensor, alpha: float = 1.0,
+                 tb: bool = False, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    with torch.no_grad():
+        return _ex.grouped_gemm(alpha, a, b, group_sizes, transB=tb, out_dtype=out_dtype)
+
+
+@grouped_gemm.register_fake
+def _(a, b, group_sizes, alpha=1.0, tb=False, out_dtype=None):
+    torch._check(a.shape[1] == b.shape[2 if tb else 1], lambda: "trnblas::grouped_gemm: inner dimensions differ")
+    return a.new_empty((a.shape[0], b.shape[1 if tb else 2]), dtype=out_dtype or a.dtype)
+
+
+def _grouped_setup(ctx, inputs, output):
+    a, b, sizes, alpha, tb, _ = inputs
+    ctx.save_for_backward(a, b, sizes)
+    ctx.alpha, ctx.tb = alpha, tb
+
+
+def _grouped_backward(ctx, d):
+    a, b, sizes = ctx.saved_tensors
+    y = d.to(a.dtype)
+    da = db = None
+    if ctx.needs_input_grad[0]:
+        da = torch.ops.trnblas.grouped_gemm(y, b, sizes, ctx.alpha, not ctx.tb, None)
+    if ctx.needs_input_grad[1]:
+        l, r = (y, a) if ctx.tb else (a, y)
+        db = torch.ops.trnblas.grouped_gemm_wgrad(l, r, sizes, ctx.alpha, None)
+    return da, db, None, None, None, None
+
+
+grouped_gemm.register_autograd(_grouped_backward, setup_context=_grouped_setup)
+
+
+@torch.library.custom_op("trnblas::grouped_gemm_wgrad", mutates_args=(), device_types="cuda")
+def grouped_gemm_wgrad(a: torch.Tensor, b: torch.Tensor, group_sizes: torch.Tensor, alpha: float = 1.0,
+                       out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    return _ex.grouped_gemm_wgrad(alpha, a, b, group_sizes, out_dtype=out_dtype)
+
+
+@grouped_gemm_wgrad.register_fake
+def _(a, b, group_sizes, alpha=1.0, out_dtype=None):
+    return a.new_empty((group_sizes.shape[0], a.shape[1], b.shape[1]), dtype=out_dtype or a.dtype)
+
+
+@torch.library.custom_op("trnblas::quantize_mxfp4", mutates_args=(), device_types="cuda")
+def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    q = _mx.quantize_mxfp4(x)
+    return q.data, q.scales
+
+
+@quantize_mxfp4.register_fake
+def _(x):
+    return (x.new_empty((*x.shape[:-1], (x.shape[-1] + 31) // 32 * 16), dtype=torch.uint8),
+            x.new_empty(_mx._scale_shape(x.shape), dtype=torch.uint8))
+
+
+@torch.library.custom_op("trnblas::dequantize_mxfp4", mutates_args=(), device_types="cuda")
+def dequantize_mxfp4(data: torch.Tensor, scales: torch.Tensor, k: int, dtype: torch.dtype) -> torch.Tensor:
+    return _mx.dequantize_mxfp4(_mx.MXFP4Tensor(data, scales, (*data.shape[:-1], k)), dtype)
+
+
+@dequantize_mxfp4.register_fake
+def _(data, scales, k, dtype):
+    return data.new_empty((*data.shape[:-1], k), dtype=dtype)
+
+
+@torch.library.custom_op("trnblas::gemm_mxfp4", mutates_args=(), device_types="cuda")
+def gemm_mxfp4(x: torch.Tensor, b_data: torch.Tensor, b_scales: torch.Tensor, alpha: float = 1.0,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    b = _mx.MXFP4Tensor(b_data, b_scales, (b_data.shape[0], x.shape[1]))
+    return _mx.gemm_mxfp4(alpha, x, b, out_dtype=out_dtype)
+
+
+@gemm_mxfp4.register_fake
+def _(x, b_data, b_scales, alpha=1.0, out_dtype=torch.bfloat16):
+    return x.new_empty((x.shape[0], b_data.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("trnblas::grouped_gemm_mxfp4", mutates_args=(), device_types="cuda")
+def grouped_gemm_mxfp4(x: torch.Tensor, b_data: torch.Tensor, b_scales: torch.Tensor, group_sizes: torch.Tensor,
+                       alpha: float = 1.0, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    b = _mx.MXFP4Tensor(b_data, b_scales, (b_data.shape[0], b_data.shape[1], x.shape[1]))
+    return _mx.grouped_gemm_mxfp4(alpha, x, b, group_sizes, out_dtype=out_dtype)
+
+
+@grouped_gemm_mxfp4.register_fake
+def _(x, b_data, b_scales, group_sizes, alpha=1.0, out_dtype=torch.bfloat16):
+    return x.new_empty((x.shape[0], b_data.shape[1]), dtype=out_dtype)
+
+
+EXPERT_OPS = {"grouped_gemm": grouped_gemm, "grouped_gemm_wgrad": grouped_gemm_wgrad,
+              "quantize_mxfp4": quantize_mxfp4, "dequantize_mxfp4": dequantize_mxfp4, "gemm_mxfp4": gemm_mxfp4,
+              "grouped_gemm_mxfp4": grouped_gemm_mxfp4}
+
+__all__ += ["EXPERT_OPS", *EXPERT_OPS]
