@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
       if (e.m) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acce_leader + static_cast<uint32_t>(buf) * 8u);
+        if (lane == 0) mbar_arrive_cluster_relaxed(acce_leader + static_cast<uint32_t>(buf) * 8u);
       }
     }
     tma_store_wait_all();
