@@ -172,11 +172,14 @@ int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t g
   const int64_t sd = groups > 1 ? strideD : round_up(ldd * M, 8);
   w.tma_d = !has_c && (reinterpret_cast<uintptr_t>(D) & 15) == 0 && (ldd * oes) % 16 == 0 && (sd * oes) % 16 == 0;
   md = ma;
-  if (w.tma_d && !encode_map_3d(&md,
-                                out_dtype == TRNBLAS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                : out_dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                                oes, D, N, M, groups, ldd, sd, 128 / oes, 32))
+  const uint64_t ddims[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(groups)};
+  const uint64_t dstrides[2] = {static_cast<uint64_t>(ldd), static_cast<uint64_t>(sd)};
+  const uint32_t dbox[3] = {static_cast<uint32_t>(64 / oes), 32, 1};
+  if (w.tma_d && !encode_map(&md,
+                             out_dtype == TRNBLAS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                             : out_dtype == TRNBLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             oes, D, 3, ddims, dstrides, dbox, CU_TENSOR_MAP_SWIZZLE_64B))
     return TRNBLAS_ERR_ALIGN;
   if (int rc = smem_attribute(reinterpret_cast<const void*>(&wgrad_pair_kernel), WgradPairCfg::SMEM, pair_attr_set))
     return rc;

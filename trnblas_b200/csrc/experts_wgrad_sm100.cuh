@@ -322,16 +322,18 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
 // completes on a barrier of each CTA, the CTA's fixer warp clears what lies
 // behind the group, and the leader's passes the stage on when both are done (a
 // fixer in the path of every stage, with its arrival at another CTA, ran at half
-// the speed). The epilogue writes 32-row blocks of 128 bytes through shared
-// memory with TMA stores: stored by lanes, a block's 32 rows cost 32 partial
-// lines an instruction, and groups of few rows are bound by their stores.
+// the speed). Eight epilogue warps, two a TMEM lane quarter, write 32-row blocks
+// of 64 bytes through shared memory with TMA stores: stored by lanes, a block's
+// 32 rows cost 32 partial lines an instruction, and groups of few rows are bound
+// by their stores (16 groups of 128 rows, 2048 x 4096: 65 us, four warps 81).
 // ---------------------------------------------------------------------------
 struct WgradPairCfg {
   static constexpr int BM = 256, BN = 256, BK = 64, STAGES = 6;
   static constexpr int A_TILE = 128 * 128, B_TILE = 128 * 128;
   static constexpr int STAGE_BYTES = A_TILE + B_TILE;
-  static constexpr int EPI = 4 * 4096;
-  static constexpr int THREADS = 32 * 7;  // producer, MMA, 4 epilogue, fixer
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int EPI = EPI_WARPS * 2048;
+  static constexpr int THREADS = 32 * (3 + EPI_WARPS);  // producer, MMA, fixer, epilogue
   static constexpr int SMEM = STAGES * STAGE_BYTES + EPI + 1024 + 512 + (kMaxGroups + 2) * 8;
 };
 
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&accf_bar[a], 1);
-      mbar_init(&acce_bar[a], 8);
+      mbar_init(&acce_bar[a], 2 * Cfg::EPI_WARPS);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 6) {
+  } else if (warp == 2) {
     // ------------------------------------------------------------ fixer (both CTAs)
     // Stages pass in the producer's order; the tail barriers' phases count the
     // uses of each stage by a cut block (one bit a stage).
@@ -572,82 +574,83 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
       }
       if (++stage == STAGES) stage = 0;
     }
-  } else if (warp >= 2 && warp < 6) {
+  } else if (warp >= 3) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
+    const int half = 128 * ((warp - 3) >> 2);  // this warp's columns of the tile
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     const uint32_t acce_leader = mapa_shared(smem_u32(acce_bar), 0);
-    uint8_t* st = epi + (warp - 2) * 4096;
+    uint8_t* st = epi + (warp - 3) * 2048;
+    // 64-byte rows: the 16-byte piece i of row l at i ^ (l / 2 & 3), the map's swizzle
+    uint4* row = reinterpret_cast<uint4*>(st + lane * 64);
+    const int swz = (lane >> 1) & 3;
     int tc = 0;
     for (int k = 0, t; (t = static_cast<int>(snake_tile(k, pair, npairs))) < p.num_tiles; ++k) {
       const Tile e = tile(t);
       const int m0 = e.m0 + 128 * rank + 32 * q;  // this warp's first row
       const int buf = tc & 1;
+      const uint32_t acc = lane_base + buf * Cfg::BN;
       if (e.m) {
         if (!mbar_wait_warp(&accf_bar[buf], (tc >> 1) & 1, ab, kTimeoutAccFull)) break;
         ++tc;
         tc_fence_after();
       }
-      auto load = [&](int c, float (&f)[32]) {
-        uint32_t v[32];
-        if (e.m) {
-          tmem_ld32(lane_base + buf * Cfg::BN + c, v);
+      const int cols = w.tma_d && p.out_kind == kOutF32 ? 16 : 32;
+#pragma unroll 1
+      for (int c = half; c < half + 128; c += cols) {
+        float f[32];
+        if (!e.m) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = 0.0f;
+        } else if (cols == 16) {
+          uint32_t v[16];
+          tmem_ld16(acc + c, v);
           tmem_ld_wait();
-        }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = e.m ? u2f(v[j]) : 0.0f;
-      };
-      if (!w.tma_d) {
-#pragma unroll 1
-        for (int c = 0; c < Cfg::BN; c += 32) {
-          float f[32];
-          load(c, f);
+          for (int j = 0; j < 16; ++j) f[j] = u2f(v[j]);
+        } else {
+          uint32_t v[32];
+          tmem_ld32(acc + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = u2f(v[j]);
+        }
+        if (!w.tma_d) {
           if (e.n0 + c < p.N) epilogue_row32(p, e.g, m0 + lane, e.n0 + c, f);
+          continue;
         }
-      } else {
-        // 128-byte rows: 32 columns of fp32, 64 of 16 bits; the 16-byte piece
-        // i of row l at i ^ (l & 7), the map's swizzle
-        const int cols = p.out_kind == kOutF32 ? 32 : 64;
-#pragma unroll 1
-        for (int c = 0; c < Cfg::BN; c += cols) {
-          tma_store_wait_read<0>();  // the last chunk's store has left the block
-          __syncwarp();
-          uint4* row = reinterpret_cast<uint4*>(st + lane * 128);
-          for (int h = 0; h < cols; h += 32) {
-            float f[32];
-            load(c + h, f);
+        tma_store_wait_read<0>();  // the last chunk's store has left the block
+        __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
-            if (p.out_kind == kOutF32) {
+        for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
+        if (cols == 16) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                row[i ^ (lane & 7)] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
-                                                 __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
-            } else {
+          for (int i = 0; i < 4; ++i)
+            row[i ^ swz] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
+                                      __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+        } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t u[4];
+          for (int i = 0; i < 4; ++i) {
+            uint32_t u[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float lo = f[8 * i + 2 * k], hi = f[8 * i + 2 * k + 1];
-                  if (p.out_kind == kOutBF16) {
-                    __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
-                    u[k] = *reinterpret_cast<uint32_t*>(&b2);
-                  } else {
-                    __half2 h2 = __floats2half2_rn(lo, hi);
-                    u[k] = *reinterpret_cast<uint32_t*>(&h2);
-                  }
-                }
-                row[(h / 8 + i) ^ (lane & 7)] = make_uint4(u[0], u[1], u[2], u[3]);
+            for (int h = 0; h < 4; ++h) {
+              const float lo = f[8 * i + 2 * h], hi = f[8 * i + 2 * h + 1];
+              if (p.out_kind == kOutBF16) {
+                __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
+                u[h] = *reinterpret_cast<uint32_t*>(&b2);
+              } else {
+                __half2 h2 = __floats2half2_rn(lo, hi);
+                u[h] = *reinterpret_cast<uint32_t*>(&h2);
               }
             }
+            row[i ^ swz] = make_uint4(u[0], u[1], u[2], u[3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (m0 < p.M && e.n0 + c < p.N) tma_store_3d(&map_d, st, e.n0 + c, m0, e.g);
-            tma_store_commit();
-          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (m0 < p.M && e.n0 + c < p.N) tma_store_3d(&map_d, st, e.n0 + c, m0, e.g);
+          tma_store_commit();
         }
       }
       if (e.m) {
