@@ -134,36 +134,28 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN, NBUF>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
-  if (Cfg::MX && p.after_quantise) wait_prerequisites();
-
   const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
   const int num_tiles = tb.tile0[p.groups + 1];
   const int work_tiles = num_kb ? tb.tile0[p.groups] : 0;
 
   if (warp == 0) {
     if (elect_one()) {
-    // ------------------------------------------------------------ producer
-    const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
-    int stage = 0;
-    uint32_t phase = 0;
-    const bool aborted = [&] {
-    for (int t = pair; t < work_tiles; t += npairs) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, t);
-      const int half = ((e.nv + 31) & ~31) / 2;  // rows of each CTA
+      // ---------------------------------------------------------- producer
+      const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      auto half_rows = [](const ExpTile& e) { return ((e.nv + 31) & ~31) / 2; };  // of each CTA
       // above three quarters one full box, else boxes of 32 rows
-      const int boxes = half > Cfg::HN * 3 / 4 ? 0 : (half + 31) / 32;
-      const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * 32 * 128 : Cfg::X_TILE);
-      const int n0 = e.n0 + 128 * rank, r0 = e.r0 + half * rank;
-      const int gw = p.w_shared ? 0 : e.g;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
-          return true;
-        }
-        if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * bytes);
-        const uint32_t fb = full_leader + static_cast<uint32_t>(stage) * 8u;
-        uint8_t* sw = smem + stage * SB;
-        uint8_t* sx = sw + Cfg::W_TILE;
+      auto row_boxes = [](int half) { return half > Cfg::HN * 3 / 4 ? 0 : (half + 31) / 32; };
+      auto load_weights = [&](const ExpTile& e, int boxes, int kb, int st) {
+        if (rank == 0)
+          mbar_arrive_expect_tx(&full_bar[st], 2 * (Cfg::W_TILE + Cfg::SFW + Cfg::SFX +
+                                                    (boxes ? boxes * 32 * 128 : Cfg::X_TILE)));
+        const uint32_t fb = full_leader + static_cast<uint32_t>(st) * 8u;
+        uint8_t* sw = smem + st * SB;
         const int k0 = kb * (Cfg::MX ? 128 : 64);  // elements of the map
+        const int n0 = e.n0 + 128 * rank;
+        const int gw = p.w_shared ? 0 : e.g;
         if (Cfg::MX || !p.w_mn) {
           tma_load_3d_pair(sw, &map_w, fb, k0, n0, gw);
         } else if (p.w_mn == 2) {
@@ -172,38 +164,65 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN, NBUF>::THREADS, 1)
           tma_load_3d_pair(sw, &map_w, fb, n0, k0, gw);
           tma_load_3d_pair(sw + 8192, &map_w, fb, n0 + 64, k0, gw);
         }
+        if constexpr (Cfg::MX)
+          tma_load_3d_pair(sw + Cfg::W_TILE + Cfg::X_TILE, &map_sw, fb, 0, 2 * kb, e.g * p.w_blocks + (n0 >> 7));
+      };
+      auto load_rows = [&](const ExpTile& e, int half, int boxes, int kb, int st) {
+        const uint32_t fb = full_leader + static_cast<uint32_t>(st) * 8u;
+        uint8_t* sx = smem + st * SB + Cfg::W_TILE;
+        const int k0 = kb * (Cfg::MX ? 128 : 64), r0 = e.r0 + half * rank;
         if (boxes == 0) tma_load_3d_pair(sx, &map_x, fb, k0, r0, 0);
         for (int j = 0; j < boxes; ++j) tma_load_3d_pair(sx + j * 4096, &map_x32, fb, k0, r0 + 32 * j, 0);
-        if constexpr (Cfg::MX) {
-          uint8_t* sf = sx + Cfg::X_TILE;
-          tma_load_3d_pair(sf, &map_sw, fb, 0, 2 * kb, e.g * p.w_blocks + (n0 >> 7));
-          tma_load_3d_pair(sf + Cfg::SFW, &map_sx, fb, 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
+        if constexpr (Cfg::MX)
+          tma_load_3d_pair(sx + Cfg::X_TILE + Cfg::SFW, &map_sx, fb, 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
+      };
+      // The weights of the first stages need not wait for the quantiser.
+      int ahead = 0;
+      if (Cfg::MX && p.after_quantise) {
+        if (pair < work_tiles) {
+          const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, pair);
+          ahead = min(STAGES, num_kb);
+          for (int kb = 0; kb < ahead; ++kb) load_weights(e, row_boxes(half_rows(e)), kb, kb);
         }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+        wait_prerequisites();
+      }
+      const bool aborted = [&] {
+        for (int t = pair; t < work_tiles; t += npairs) {
+          const ExpTile e = exp_tile<BN, Cfg::STEP, 256>(tb, p.groups, p.tiles_w, t);
+          const int half = half_rows(e), boxes = row_boxes(half);
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (ahead > 0) {
+              --ahead;
+            } else {
+              if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) return true;
+              load_weights(e, boxes, kb, stage);
+            }
+            load_rows(e, half, boxes, kb, stage);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        return false;
+      }();
+      if (aborted || ab.raised()) {
+        // copies already issued complete on the leader's barriers, which this
+        // CTA cannot observe: give them time to land (bounded)
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000000ull) {
+        }
+      } else {
+        // wait until the MMA has released every stage, so that no commit is in
+        // flight towards this CTA when it passes the exit barrier
+        for (int i = 0; i < STAGES; ++i) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) break;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
-    }
-      return false;
-    }();
-    if (aborted || ab.raised()) {
-      // copies already issued complete on the leader's barriers, which this
-      // CTA cannot observe: give them time to land (bounded)
-      const unsigned long long t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 20000000ull) {
-      }
-    } else {
-      // wait until the MMA has released every stage, so that no commit is in
-      // flight towards this CTA when it passes the exit barrier
-      for (int i = 0; i < STAGES; ++i) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) break;
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
     }
     __syncwarp();
   } else if (warp == 1 && rank == 0) {

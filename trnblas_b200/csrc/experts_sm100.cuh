@@ -360,8 +360,6 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
-  if (Cfg::MX && p.after_quantise) wait_prerequisites();
-
   const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
   const int num_tiles = tb.tile0[p.groups + 1];
   // tiles with products; the ones behind are stores of beta * C alone
@@ -369,60 +367,79 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
 
   if (warp == 0) {
     if (elect_one()) {
-    // ------------------------------------------------------------ producer
-    int stage = 0;
-    uint32_t phase = 0;
-    const bool aborted = [&] {
-    for (int t = blockIdx.x; t < work_tiles; t += gridDim.x) {
-      const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
-      // above three quarters of the tile one full box, else small boxes
-      const int boxes = e.nv > BN * 3 / 4 ? 0 : (e.nv + Cfg::XBOX - 1) / Cfg::XBOX;
-      const uint32_t bytes = Cfg::W_TILE + Cfg::SFW + Cfg::SFX + (boxes ? boxes * Cfg::XBOX * 128 : Cfg::X_TILE);
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
-          return true;
-        }
-        uint8_t* sw = smem + stage * SB;
-        uint8_t* sx = sw + Cfg::W_TILE;
-        mbar_arrive_expect_tx(&full_bar[stage], bytes);
+      // ---------------------------------------------------------- producer
+      int stage = 0;
+      uint32_t phase = 0;
+      // above three quarters of the tile one full box of rows, else small boxes
+      auto row_boxes = [](const ExpTile& e) {
+        return e.nv > BN * 3 / 4 ? 0 : (e.nv + Cfg::XBOX - 1) / Cfg::XBOX;
+      };
+      auto load_weights = [&](const ExpTile& e, int boxes, int kb, int st) {
+        uint8_t* sw = smem + st * SB;
+        uint64_t* bar = &full_bar[st];
+        mbar_arrive_expect_tx(bar, Cfg::W_TILE + Cfg::SFW + Cfg::SFX +
+                                       (boxes ? boxes * Cfg::XBOX * 128 : Cfg::X_TILE));
         if constexpr (Cfg::MX) {
-          const int k0 = kb * 128;  // bytes
-          tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, e.g);
-          if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
-          for (int j = 0; j < boxes; ++j)
-            tma_load_3d(sx + j * Cfg::XBOX * 128, &map_xs, &full_bar[stage], k0, e.r0 + Cfg::XBOX * j, 0);
-          uint8_t* sf = sx + Cfg::X_TILE;
-          tma_load_3d(sf, &map_sw, &full_bar[stage], 0, 2 * kb, e.g * p.w_blocks + (e.n0 >> 7));
-          tma_load_3d(sf + Cfg::SFW, &map_sx, &full_bar[stage], 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
+          tma_load_3d(sw, &map_w, bar, kb * 128, e.n0, e.g);  // (bytes)
+          tma_load_3d(sw + Cfg::W_TILE + Cfg::X_TILE, &map_sw, bar, 0, 2 * kb, e.g * p.w_blocks + (e.n0 >> 7));
         } else {
-          const int k0 = kb * Cfg::BK;
-          const int gw = p.w_shared ? 0 : e.g;
+          const int k0 = kb * Cfg::BK, gw = p.w_shared ? 0 : e.g;
           if (!p.w_mn) {
-            tma_load_3d(sw, &map_w, &full_bar[stage], k0, e.n0, gw);
+            tma_load_3d(sw, &map_w, bar, k0, e.n0, gw);
           } else if (p.w_mn == 2) {
-            tma_load_4d(sw, &map_w, &full_bar[stage], 0, k0, e.n0 >> 6, gw);
+            tma_load_4d(sw, &map_w, bar, 0, k0, e.n0 >> 6, gw);
           } else {
-            tma_load_3d(sw, &map_w, &full_bar[stage], e.n0, k0, gw);
-            tma_load_3d(sw + 8192, &map_w, &full_bar[stage], e.n0 + 64, k0, gw);
+            tma_load_3d(sw, &map_w, bar, e.n0, k0, gw);
+            tma_load_3d(sw + 8192, &map_w, bar, e.n0 + 64, k0, gw);
           }
-          if (boxes == 0) tma_load_3d(sx, &map_x, &full_bar[stage], k0, e.r0, 0);
-          for (int j = 0; j < boxes; ++j)
-            tma_load_3d(sx + j * Cfg::XBOX * 128, &map_xs, &full_bar[stage], k0, e.r0 + Cfg::XBOX * j, 0);
         }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+      };
+      auto load_rows = [&](const ExpTile& e, int boxes, int kb, int st) {
+        uint8_t* sx = smem + st * SB + Cfg::W_TILE;
+        uint64_t* bar = &full_bar[st];
+        const int k0 = kb * (Cfg::MX ? 128 : 64);
+        if (boxes == 0) tma_load_3d(sx, &map_x, bar, k0, e.r0, 0);
+        for (int j = 0; j < boxes; ++j)
+          tma_load_3d(sx + j * Cfg::XBOX * 128, &map_xs, bar, k0, e.r0 + Cfg::XBOX * j, 0);
+        if constexpr (Cfg::MX)
+          tma_load_3d(sx + Cfg::X_TILE + Cfg::SFW, &map_sx, bar, 0, 2 * kb, tb.blk0[e.g] + (e.x0 >> 7));
+      };
+      // The weights of the first stages need not wait for the quantiser.
+      int ahead = 0;
+      if (Cfg::MX && p.after_quantise) {
+        if (static_cast<int>(blockIdx.x) < work_tiles) {
+          const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, blockIdx.x);
+          ahead = min(STAGES, num_kb);
+          for (int kb = 0; kb < ahead; ++kb) load_weights(e, row_boxes(e), kb, kb);
+        }
+        wait_prerequisites();
+      }
+      const bool aborted = [&] {
+        for (int t = blockIdx.x; t < work_tiles; t += gridDim.x) {
+          const ExpTile e = exp_tile<BN, Cfg::STEP>(tb, p.groups, p.tiles_w, t);
+          const int boxes = row_boxes(e);
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (ahead > 0) {
+              --ahead;
+            } else {
+              if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) return true;
+              load_weights(e, boxes, kb, stage);
+            }
+            load_rows(e, boxes, kb, stage);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        return false;
+      }();
+      if (aborted || ab.raised()) {
+        // let copies already issued land before the CTA exits (bounded)
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000000ull) {
         }
       }
-    }
-      return false;
-    }();
-    if (aborted || ab.raised()) {
-      // let copies already issued land before the CTA exits (bounded)
-      const unsigned long long t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 20000000ull) {
-      }
-    }
     }
     __syncwarp();
   } else if (warp == 1) {

@@ -134,38 +134,37 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
 
   if (warp == 0) {
     if (elect_one()) {
-    // ------------------------------------------------------------ producer
-    int stage = 0;
-    uint32_t phase = 0;
-    const bool aborted = [&] {
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles; ++k) {
-      const Tile e = tile(t);
-      for (int r = 0; r < e.m; r += Cfg::BK) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) {
-          return true;
+      // ---------------------------------------------------------- producer
+      int stage = 0;
+      uint32_t phase = 0;
+      const bool aborted = [&] {
+        for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles; ++k) {
+          const Tile e = tile(t);
+          for (int r = 0; r < e.m; r += Cfg::BK) {
+            if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) return true;
+            uint8_t* sa = smem + stage * SB;
+            uint8_t* sb = sa + Cfg::A_TILE;
+            mbar_arrive_expect_tx(&full_bar[stage], SB);
+#pragma unroll
+            for (int j = 0; j < Cfg::BM / 64; ++j)
+              tma_load_3d(sa + j * 8192, &map_a, &full_bar[stage], e.m0 + 64 * j, e.r0 + r, 0);
+#pragma unroll
+            for (int j = 0; j < Cfg::BN / 64; ++j)
+              tma_load_3d(sb + j * 8192, &map_b, &full_bar[stage], e.n0 + 64 * j, e.r0 + r, 0);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
         }
-        uint8_t* sa = smem + stage * SB;
-        uint8_t* sb = sa + Cfg::A_TILE;
-        mbar_arrive_expect_tx(&full_bar[stage], SB);
-#pragma unroll
-        for (int j = 0; j < Cfg::BM / 64; ++j)
-          tma_load_3d(sa + j * 8192, &map_a, &full_bar[stage], e.m0 + 64 * j, e.r0 + r, 0);
-#pragma unroll
-        for (int j = 0; j < Cfg::BN / 64; ++j)
-          tma_load_3d(sb + j * 8192, &map_b, &full_bar[stage], e.n0 + 64 * j, e.r0 + r, 0);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+        return false;
+      }();
+      if (aborted || ab.raised()) {
+        // let copies already issued land before the CTA exits (bounded)
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000000ull) {
         }
       }
-    }
-      return false;
-    }();
-    if (aborted || ab.raised()) {
-      const unsigned long long t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 20000000ull) {
-      }
-    }
     }
     __syncwarp();
   } else if (warp == 1) {
