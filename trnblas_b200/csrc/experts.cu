@@ -59,11 +59,8 @@ int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups,
   const bool shared = groups == 1 || strideB == 0;  // one matrix
   const int64_t nb = shared ? 1 : groups, sb = shared ? round_up(ldb * b_rows, 8) : strideB;
   const int64_t sa = round_up(lda * rows, 8);
-  // Row tiles of 64 where a group has at most 48 rows on average: eight
-  // pipeline stages instead of four keep more weight bytes in flight, which is
-  // what bounds a few rows a group. Longer groups go to CTA pairs when there
-  // are weight columns for both.
-  const bool small = rows <= 48 * groups;
+  // Longer groups go to CTA pairs when there are weight columns for both.
+  const bool small = small_tiles(rows, groups, N, true);
   const bool pair = !small && N > 128;
   const bool wide = !transB && N % 64 == 0;  // both 64-column blocks in one copy
   CUtensorMap mw, mx, mxs;

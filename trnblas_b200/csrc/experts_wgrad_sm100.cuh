@@ -5,35 +5,6 @@
 
 namespace tb {
 
-// Groups by falling length (all threads of the block; `order` in shared memory):
-// the walk takes a group's tiles one round of CTAs after another, so with the
-// longest first, and every other round backwards (snake_tile), the CTAs end
-// within about one short tile of each other. Without it one long group's tiles
-// fall twice to some CTAs and once to others (16 skewed groups of 16384 rows,
-// 4096 x 2048: 259 us against the figure at the kernel). More than kSortGroups groups keep
-// their order: there the differences average out.
-constexpr int kSortGroups = 128;
-
-__device__ __forceinline__ void order_groups(const int* row0, int groups, int* order) {
-  for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-    int rank = g;
-    if (groups <= kSortGroups) {
-      const int m = row0[g + 1] - row0[g];
-      rank = 0;
-      for (int j = 0; j < groups; ++j) {
-        const int n = row0[j + 1] - row0[j];
-        rank += n > m || (n == m && j < g);
-      }
-    }
-    order[rank] = g;
-  }
-}
-
-// The k-th tile of walker `w` of `n`.
-__device__ __forceinline__ long long snake_tile(int k, int w, int n) {
-  return static_cast<long long>(k) * n + ((k & 1) ? n - 1 - w : w);
-}
-
 // ---------------------------------------------------------------------------
 // Weight gradient: D[g] (M x N) = alpha * A_g^T B_g + beta * C[g], A_g the
 // group's rows of A (rows x M), B_g of B (rows x N), both read MN-major in
@@ -59,7 +30,7 @@ struct WgradCfg {
   static constexpr int STAGE_BYTES = A_TILE + B_TILE;
   static constexpr int TMEM_COLS = 512;
   static constexpr int THREADS = 32 * 7;  // producer, MMA, 4 epilogue, fixer
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + (kMaxGroups + 2) * 8;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + (kMaxGroups + 2) * 4;
 };
 
 __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
@@ -84,7 +55,6 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
   GroupTable tb;
   tb.row0 = reinterpret_cast<int*>(smem + STAGES * SB + 512);
   tb.tile0 = tb.blk0 = nullptr;
-  int* order = tb.row0 + kMaxGroups + 2;
 
   const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -111,8 +81,6 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
   if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
-  order_groups(tb.row0, w.groups, order);
-  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
@@ -122,9 +90,8 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
   };
   auto tile = [&](int t) -> Tile {
     Tile e;
-    const int s = t / per_group;
-    const int i = t - s * per_group;
-    e.g = order[s];
+    e.g = t / per_group;
+    const int i = t - e.g * per_group;
     e.m0 = (i % p.tiles_m) * Cfg::BM;
     e.n0 = (i / p.tiles_m) * Cfg::BN;
     e.r0 = tb.row0[e.g];
@@ -138,7 +105,7 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       const bool aborted = [&] {
-        for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles; ++k) {
+        for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
           const Tile e = tile(t);
           for (int r = 0; r < e.m; r += Cfg::BK) {
             if (!mbar_wait(&empty_bar[stage], phase ^ 1u, ab, kTimeoutEmpty)) return true;
@@ -183,7 +150,7 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
     }
     int stage = 0, tc = 0;
     uint32_t phase = 0;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles; ++k) {
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
       const int m = warp_uniform(tile(t).m);
       if (m == 0) continue;
       const int buf = tc & 1;
@@ -238,7 +205,7 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
     int stage = 0;
     uint32_t phase = 0;
     bool stop = false;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles && !stop; ++k) {
+    for (int t = blockIdx.x; t < p.num_tiles && !stop; t += gridDim.x) {
       const Tile e = tile(t);
       for (int r = 0; r < e.m; r += Cfg::BK) {
         if (!mbar_wait_warp(&full_bar[stage], phase, ab, kTimeoutAux)) {
@@ -269,7 +236,7 @@ __global__ void __launch_bounds__(WgradCfg::THREADS, 1)
     const int q = warp & 3;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     int tc = 0;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, blockIdx.x, gridDim.x))) < p.num_tiles; ++k) {
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x) {
       const Tile e = tile(t);
       const int r = e.m0 + 32 * q + lane;
       const int buf = tc & 1;
@@ -333,7 +300,7 @@ struct WgradPairCfg {
   static constexpr int EPI_WARPS = 8;
   static constexpr int EPI = EPI_WARPS * 2048;
   static constexpr int THREADS = 32 * (3 + EPI_WARPS);  // producer, MMA, fixer, epilogue
-  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI + 1024 + 512 + (kMaxGroups + 2) * 8;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI + 1024 + 512 + (kMaxGroups + 2) * 4;
 };
 
 __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
@@ -360,7 +327,6 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
   GroupTable tb;
   tb.row0 = reinterpret_cast<int*>(epi + Cfg::EPI + 512);
   tb.tile0 = tb.blk0 = nullptr;
-  int* order = tb.row0 + kMaxGroups + 2;
 
   const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -392,8 +358,6 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  order_groups(tb.row0, w.groups, order);
-  __syncthreads();
   __syncwarp();
   cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
   tc_fence_after();
@@ -405,9 +369,8 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
   };
   auto tile = [&](int t) -> Tile {
     Tile e;
-    const int s = t / per_group;
-    const int i = t - s * per_group;
-    e.g = order[s];
+    e.g = t / per_group;
+    const int i = t - e.g * per_group;
     e.m0 = (i % p.tiles_m) * Cfg::BM;
     e.n0 = (i / p.tiles_m) * Cfg::BN;
     e.r0 = tb.row0[e.g];
@@ -425,7 +388,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       const bool aborted = [&] {
-        for (int k = 0, t; (t = static_cast<int>(snake_tile(k, pair, npairs))) < p.num_tiles; ++k) {
+        for (int t = pair; t < p.num_tiles; t += npairs) {
           const Tile e = tile(t);
           const int m0 = e.m0 + 128 * rank, n0 = e.n0 + 128 * rank;
           for (int r = 0; r < e.m; r += Cfg::BK) {
@@ -489,7 +452,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
     const uint32_t id = idesc(kAccF32, w.in_fmt, w.in_fmt, 1, 1, Cfg::BM, Cfg::BN);
     int stage = 0, tc = 0;
     uint32_t phase = 0;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, pair, npairs))) < p.num_tiles; ++k) {
+    for (int t = pair; t < p.num_tiles; t += npairs) {
       const int m = warp_uniform(tile(t).m);
       if (m == 0) continue;
       const int buf = tc & 1;
@@ -546,7 +509,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
     const uint32_t peer_leader = mapa_shared(smem_u32(peer_bar), 0);
     int stage = 0;
     uint32_t tphase = 0;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, pair, npairs))) < p.num_tiles; ++k) {
+    for (int t = pair; t < p.num_tiles; t += npairs) {
       const int m = warp_uniform(tile(t).m);
       const int blocks = (m + Cfg::BK - 1) / Cfg::BK;
       if (blocks == 0) continue;
@@ -584,7 +547,7 @@ __global__ void __launch_bounds__(WgradPairCfg::THREADS, 1)
     uint4* row = reinterpret_cast<uint4*>(st + lane * 64);
     const int swz = (lane >> 1) & 3;
     int tc = 0;
-    for (int k = 0, t; (t = static_cast<int>(snake_tile(k, pair, npairs))) < p.num_tiles; ++k) {
+    for (int t = pair; t < p.num_tiles; t += npairs) {
       const Tile e = tile(t);
       const int m0 = e.m0 + 128 * rank + 32 * q;  // this warp's first row
       const int buf = tc & 1;
