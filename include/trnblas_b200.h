@@ -262,26 +262,34 @@ TRNBLAS_API int trnblas_pair_energy(int64_t nocc, int64_t nvir, int64_t naux, co
  * synchronisation, any of them may be zero. Negative sizes count as zero and
  * sizes beyond `rows` are cut off; both leave code 8 in the status word. At
  * most 1024 groups. The gradient of A is the same call on D's gradient with
- * transB flipped. No workspace; D must not overlap A, B or C.
+ * transB flipped. Operands off 16 bytes (base, row stride or matrix stride) are
+ * copied into the workspace first, whose size the first function gives (0
+ * otherwise). D must not overlap A, B or C.
  */
+TRNBLAS_API size_t trnblas_grouped_gemm_workspace_size(int64_t rows, int64_t groups, int64_t N, int64_t K,
+                                           const void* A, int64_t lda, const void* B, int64_t ldb,
+                                           int64_t strideB, int transB);
 TRNBLAS_API int trnblas_grouped_gemm(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t N,
                          int64_t K, float alpha, const void* A, int64_t lda, const void* B,
                          int64_t ldb, int64_t strideB, int transB, const void* group_sizes,
                          int sizes_64, float beta, const void* C, int64_t ldc, void* D, int64_t ldd,
-                         void* stream);
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The gradient of trnblas_grouped_gemm's weights: D[g] = alpha * A_g^T @ B_g +
  * beta * C[g], A_g (B_g) the rows of group g of the rows x M (rows x N)
  * operand; beta * C[g] for a group without rows. C and D are stacks of
  * `groups` M x N matrices of out_dtype. Nothing behind the last group is read
- * into a result, infinities and NaN included.
+ * into a result, infinities and NaN included. Workspace as above.
  */
+TRNBLAS_API size_t trnblas_grouped_gemm_wgrad_workspace_size(int64_t rows, int64_t M, int64_t N, const void* A,
+                                                 int64_t lda, const void* B, int64_t ldb);
 TRNBLAS_API int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t rows, int64_t groups, int64_t M,
                                int64_t N, float alpha, const void* A, int64_t lda, const void* B,
                                int64_t ldb, const void* group_sizes, int sizes_64, float beta,
                                const void* C, int64_t ldc, int64_t strideC, void* D, int64_t ldd,
-                               int64_t strideD, void* stream);
+                               int64_t strideD, void* workspace, size_t workspace_bytes,
+                               void* stream);
 
 /*
  * Microscaled 4-bit floating point (OCP MX, MXFP4): blocks of 32 values along

@@ -77,7 +77,8 @@ def test_c_entry_points_check_their_arguments():
     def grouped(**kw):
         v = {**ok, **kw}
         return L.trnblas_grouped_gemm(v["dt"], v["od"], v["rows"], v["G"], v["n"], v["k"], 1.0, v["a"], v["lda"], v["b"],
-                                      v["ldb"], v["sb"], v["tb"], v["s"], 0, 1.0, v["c"], v["ldc"], v["d"], v["ldd"], None)
+                                      v["ldb"], v["sb"], v["tb"], v["s"], 0, 1.0, v["c"], v["ldc"], v["d"], v["ldd"],
+                                      None, 0, None)
 
     for bad in (dict(dt=N.F32), dict(od=N.F16), dict(rows=-1), dict(G=1025), dict(s=None), dict(d=None), dict(ldd=7),
                 dict(a=None), dict(lda=7), dict(ldb=7), dict(sb=-8), dict(c=FAKE, ldc=7), dict(rows=1 << 31), dict(tb=1, k=16)):
@@ -88,12 +89,24 @@ def test_c_entry_points_check_their_arguments():
         v = {**ok, **kw}
         return L.trnblas_grouped_gemm_wgrad(v["dt"], v["od"], v["rows"], v["G"], v["k"], v["n"], 1.0, v["a"], v["lda"],
                                             v["b"], v["ldb"], v["s"], 0, 1.0, v["c"], v["ldc"], 64, v["d"], v["ldd"],
-                                            v["sb"], None)
+                                            v["sb"], None, 0, None)
 
     for bad in (dict(dt=N.F64), dict(od=N.F16), dict(G=-1), dict(s=None), dict(d=None), dict(ldd=7), dict(a=None),
                 dict(lda=7), dict(ldb=7), dict(sb=63), dict(c=FAKE, ldc=7)):
         assert wgrad(**bad) == N.ERR_ARG, bad
     assert wgrad(G=0) == 0
+    # operands off 16 bytes need a workspace for their copies
+    for bad in (dict(a=FAKE + 2), dict(lda=9), dict(b=FAKE + 8), dict(ldb=12), dict(sb=68)):
+        assert grouped(**bad) == N.ERR_WORKSPACE, bad
+    for bad in (dict(a=FAKE + 2), dict(lda=9), dict(ldb=12)):
+        assert wgrad(**bad) == N.ERR_WORKSPACE, bad
+    size = L.trnblas_grouped_gemm_workspace_size
+    assert size(4, 2, 8, 8, FAKE, 8, FAKE, 8, 64, 0) == 0
+    assert size(4, 2, 8, 8, FAKE + 2, 8, FAKE, 8, 64, 0) == 256
+    assert size(100, 3, 8, 30, FAKE, 30, FAKE, 8, 240, 0) == 6400
+    assert size(100, 3, 9, 64, FAKE, 64, FAKE, 9, 576, 0) == 3 * 64 * 16 * 2
+    assert size(100, 3, 9, 64, FAKE, 64, FAKE, 9, 0, 0) == 64 * 16 * 2  # one matrix for all
+    assert L.trnblas_grouped_gemm_wgrad_workspace_size(100, 30, 8, FAKE, 30, FAKE, 8) == 6400
 
     q = L.trnblas_mxfp4_quantize
     for args in ((N.F64, 4, 8, FAKE, 8, FAKE, 16, FAKE), (N.F32, -1, 8, FAKE, 8, FAKE, 16, FAKE),

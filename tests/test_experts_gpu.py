@@ -116,6 +116,36 @@ def test_strides_and_expanded_weights():
     X.check(w, ref, X.tolerance(ref, mags, max(sizes), BF))
 
 
+@pytest.mark.parametrize("off,step", [(0, 1), (1, 1), (2, 2), (4, 4), (3, 7)])
+def test_operands_off_16_bytes(off, step):
+    """Bases and row, matrix strides of every alignment: copied, in the widest
+    pieces they allow, before the product."""
+    sizes, K, Nn = [5, 0, 70, 140], 93 + step, 61 + step
+    rows = sum(sizes) + 3
+    flat = _rand(9 * (K + 9) * (Nn + 9) + 2 * rows * (K + Nn))
+
+    def at(o, shape, strides):
+        return flat.as_strided(shape, strides, o)
+
+    A = at(off, (rows, K), (K + step, 1))
+    dD = at(off + 2, (rows, Nn), (Nn + step, 1))
+    for B, tB in ((at(off, (4, K, Nn), (K * (Nn + step) + step, Nn + step, 1)), False),
+                  (at(off, (4, Nn, K), (Nn * (K + step), K + step, 1)), True),
+                  (at(off, (4, K, Nn), (Nn * (K + step) + step, 1, K + step)), False),  # stored by columns
+                  (at(off, (1, K, Nn), (1, Nn + step, 1)).expand(4, K, Nn), False),
+                  (at(off, (4, K, Nn), (2 * K * Nn, 2 * Nn, 2)), False)):
+        ref, mags = X.grouped_gemm(1.0, A, B, sizes, transB=tB)
+        X.check(tb.grouped_gemm(1.0, A, B, _sizes(sizes), transB=tB), ref, X.tolerance(ref, mags, K, BF))
+    ref, mags = X.wgrad(1.0, A, dD, sizes)
+    X.check(tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes)), ref, X.tolerance(ref, mags, max(sizes), BF))
+    a, b = A.clone().requires_grad_(), _rand(4, K, Nn).requires_grad_()
+    da, db = torch.autograd.grad(tb.grouped_gemm(1.0, a, b, _sizes(sizes)), (a, b), dD)
+    ref, mags = X.grouped_gemm(1.0, dD, b.detach(), sizes, transB=True)
+    X.check(da, ref, X.tolerance(ref, mags, Nn, BF))
+    ref, mags = X.wgrad(1.0, A, dD, sizes)
+    X.check(db, ref, X.tolerance(ref, mags, max(sizes), BF))
+
+
 def test_sizes_on_host_64_bit_and_strided():
     sizes = [5, 0, 90]
     A, B = _rand(95, 64), _rand(3, 64, 64)

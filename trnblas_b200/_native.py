@@ -72,12 +72,17 @@ _SIGNATURES = {
     "trnblas_pair_energy": (
         _i, [_i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _sz, _p]
     ),
+    "trnblas_grouped_gemm_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _i]),
     "trnblas_grouped_gemm": (
-        _i, [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i64, _i, _p, _i, _f, _p, _i64, _p, _i64, _p]
+        _i,
+        [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i64, _i, _p, _i, _f, _p, _i64, _p, _i64, _p, _sz,
+         _p],
     ),
+    "trnblas_grouped_gemm_wgrad_workspace_size": (_sz, [_i64, _i64, _i64, _p, _i64, _p, _i64]),
     "trnblas_grouped_gemm_wgrad": (
         _i,
-        [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p, _i, _f, _p, _i64, _i64, _p, _i64, _i64, _p],
+        [_i, _i, _i64, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p, _i, _f, _p, _i64, _i64, _p, _i64, _i64, _p, _sz,
+         _p],
     ),
     "trnblas_mxfp4_quantize": (_i, [_i, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p]),
     "trnblas_mxfp4_dequantize": (_i, [_i, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p]),

@@ -15,7 +15,7 @@ import torch
 
 from . import _native as N
 from ._flags import trans_flag
-from .level3 import _add_c, _cuda_device, _flat_batch, _fuse_c, _home, _mixed_dtype_error, _tma_operand, _to
+from .level3 import _add_c, _cuda_device, _fuse_c, _home, _mixed_dtype_error, _to
 
 DTYPES = (torch.bfloat16, torch.float16)
 MAX_GROUPS = 1024
@@ -76,28 +76,30 @@ def check_group_sizes(name: str, sizes, groups: int | None, rows: int) -> None:
 
 
 def _rows_operand(x: torch.Tensor):
-    """(tensor, ld) of a rows x cols operand stored row by row on 16 bytes."""
+    """(tensor, ld) of a rows x cols operand stored row by row."""
     s0, s1 = x.stride()
-    if s1 == 1 and s0 % 8 == 0 and s0 >= x.shape[1] and x.data_ptr() % 16 == 0 and s0:
-        return x, s0
-    t, ld, tr = _tma_operand(x, x.element_size())
-    if tr:
-        t, ld, tr = _tma_operand(x.contiguous(), x.element_size())
-    if tr:  # a single column: pad its rows
-        q = 16 // x.element_size()
-        t = x.new_zeros((x.shape[0], q))
-        t[:, : x.shape[1]].copy_(x)
-        ld = q
-    return t, ld
+    rows, cols = x.shape
+    if s1 != 1 or s0 < cols:
+        x = x.contiguous()
+        if rows <= 1 or cols <= 1:  # strides of a single row or column say nothing
+            return x, cols
+        s0 = cols
+    return x, s0
 
 
 def _weights_operand(B: torch.Tensor, transB: bool):
-    """(tensor, ld, stored N x K, matrix stride) of the stack op(B) as `_flat_batch`
-    gives them; an ordinary contiguous stack needs no look at its strides."""
+    """(tensor, ld, stored N x K, matrix stride) of the stack op(B): matrices
+    stored by rows or by columns are read where they are; stride 0 is one matrix
+    for all groups."""
     G, rows, cols = B.shape
-    if G > 1 and cols % 8 == 0 and cols and B.is_contiguous() and B.data_ptr() % 16 == 0:
-        return B, cols, transB, rows * cols
-    return _flat_batch(B.mT if transB else B, (G,), B.element_size(), False)
+    s0, s1, s2 = B.stride()
+    if s2 == 1 and s1 >= cols:
+        return B, s1, transB, s0 if G > 1 else 0
+    if s1 == 1 and s2 >= rows:
+        return B, s2, not transB, s0 if G > 1 else 0
+    if G > 1 and s0 == 0:
+        return *_weights_operand(B[:1].contiguous(), transB)[:3], 0
+    return B.contiguous(), cols, transB, rows * cols
 
 
 def _c_operand(C, cols: int):
@@ -122,13 +124,17 @@ def _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype):
     c_arg, ldc = _c_operand(C, Nn) if C is not None else (None, 0)
     if not sizes.is_contiguous():
         sizes = sizes.contiguous()
+    ap, bp, ws, ws_bytes = at.data_ptr(), bt.data_ptr(), None, 0
+    if (lda | ldb | sb) & 7 or (ap | bp) & 15:  # TMA needs copies
+        ws_bytes = N.lib().trnblas_grouped_gemm_workspace_size(rows, G, Nn, K, ap, lda, bp, ldb, sb, tb)
+        ws = empty((ws_bytes,), torch.uint8, dev)
     rc = call_on(
         dev, N.lib().trnblas_grouped_gemm, N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, Nn, K, float(alpha),
-        at.data_ptr(), lda, bt.data_ptr(), ldb, sb, tb, sizes.data_ptr(), sizes.dtype == torch.int64,
-        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, out.data_ptr(), Nn)
+        ap, lda, bp, ldb, sb, tb, sizes.data_ptr(), sizes.dtype == torch.int64,
+        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, out.data_ptr(), Nn, N.ptr(ws), ws_bytes)
     if rc:
         N.check(rc, "trnblas_grouped_gemm")
-    N.count_launches(1)
+    N.count_launches(2 if ws_bytes else 1)
     return out
 
 
@@ -148,13 +154,17 @@ def _wgrad(alpha, a, b, sizes, beta, C, out_dtype):
         sc = c_arg.stride(0)
     if not sizes.is_contiguous():
         sizes = sizes.contiguous()
+    ap, bp, ws, ws_bytes = at.data_ptr(), bt.data_ptr(), None, 0
+    if (lda | ldb) & 7 or (ap | bp) & 15:  # TMA needs copies
+        ws_bytes = N.lib().trnblas_grouped_gemm_wgrad_workspace_size(rows, M, Nn, ap, lda, bp, ldb)
+        ws = empty((ws_bytes,), torch.uint8, dev)
     rc = call_on(
         dev, N.lib().trnblas_grouped_gemm_wgrad, N.dtype_code(a.dtype), N.dtype_code(out_dtype), rows, G, M, Nn, float(alpha),
-        at.data_ptr(), lda, bt.data_ptr(), ldb, sizes.data_ptr(), sizes.dtype == torch.int64,
-        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, sc, out.data_ptr(), Nn, M * Nn)
+        ap, lda, bp, ldb, sizes.data_ptr(), sizes.dtype == torch.int64,
+        float(beta) if C is not None else 0.0, N.ptr(c_arg), ldc, sc, out.data_ptr(), Nn, M * Nn, N.ptr(ws), ws_bytes)
     if rc:
         N.check(rc, "trnblas_grouped_gemm_wgrad")
-    N.count_launches(1)
+    N.count_launches(2 if ws_bytes else 1)
     return out
 
 
