@@ -174,26 +174,27 @@ class _GroupedGemm(torch.autograd.Function):
     dC = beta dD."""
 
     @staticmethod
-    def forward(ctx, alpha, a, B, transB, sizes, beta, C, out_dtype):
+    def forward(ctx, args, a, B, sizes, C):
+        alpha, transB, beta, out_dtype = ctx.args = args
         ctx.save_for_backward(a, B, sizes)
-        ctx.args = (alpha, transB, beta)
         return _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dD):
         a, B, sizes = ctx.saved_tensors
-        alpha, transB, beta = ctx.args
+        alpha, transB, beta, _ = ctx.args
+        _, need_a, need_B, _, need_C = ctx.needs_input_grad
         y = dD if dD.dtype == a.dtype else dD.to(a.dtype)
         da = dB = dC = None
-        if ctx.needs_input_grad[1]:
+        if need_a:
             da = _grouped(alpha, y, B, not transB, sizes, 0.0, None, a.dtype)
-        if ctx.needs_input_grad[2]:
+        if need_B:
             l, r = (y, a) if transB else (a, y)
             dB = _wgrad(alpha, l, r, sizes, 0.0, None, B.dtype)
-        if ctx.needs_input_grad[6]:
+        if need_C:
             dC = beta * dD
-        return None, da, dB, None, None, None, dC, None
+        return None, da, dB, None, dC
 
 
 def grouped_gemm(
@@ -237,7 +238,7 @@ def grouped_gemm(
     grad = (A.requires_grad or B.requires_grad) and torch.is_grad_enabled()
     if C is None and _same_cuda_device(A, B, group_sizes):
         if grad:
-            return _GroupedGemm.apply(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
+            return _GroupedGemm.apply((alpha, transB, 0.0, out_dtype), A, B, group_sizes, None)
         return _grouped(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)
@@ -245,7 +246,7 @@ def grouped_gemm(
     fuse = _fuse_c(Cd, beta, (a.shape[0], b.shape[1] if transB else b.shape[2]), out_dtype, dev)
     c_arg = Cd if fuse else None
     if grad or (torch.is_grad_enabled() and fuse and Cd.requires_grad):
-        r = _GroupedGemm.apply(alpha, a, b, transB, sizes, beta, c_arg, out_dtype)
+        r = _GroupedGemm.apply((alpha, transB, beta, out_dtype), a, b, sizes, c_arg)
         if not fuse and C is not None and beta != 0.0:
             r = r + beta * Cd
         return r if home == dev else r.to(home)
