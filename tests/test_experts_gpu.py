@@ -54,6 +54,36 @@ def test_grouped_gemm(sizes, transB, K, Nn):
     assert tb.device_status(0) == 0
 
 
+PAIRED = [[513, 64, 0, 255, 256, 257], [1, 0, 1290, 3], [700, 300, 129, 31, 0, 40]]
+
+
+@pytest.mark.parametrize("sizes", PAIRED, ids=lambda s: f"{len(s)}x{max(s)}")
+@pytest.mark.parametrize("transB", [False, True])
+@pytest.mark.parametrize("K,Nn", [(200, 2056), (64, 2304), (1032, 4100), (65, 2049), (7, 3000)])
+def test_grouped_gemm_on_pairs(sizes, transB, K, Nn):
+    """Enough tiles for the CTA pairs, which smaller products do not reach."""
+    dt = BF if K % 2 == 0 else FP
+    rows = sum(sizes) + (K % 3) * 150
+    A, B = _rand(rows, K, dt=dt), _rand(len(sizes), *((Nn, K) if transB else (K, Nn)), dt=dt)
+    ref, mags = X.grouped_gemm(0.5, A, B, sizes, transB=transB)
+    for out in (dt, F32):
+        D = tb.grouped_gemm(0.5, A, B, _sizes(sizes), transB=transB, out_dtype=out)
+        X.check(D, ref, X.tolerance(ref, mags, K, out), f"{sizes} {K} {Nn} {out}")
+        C = _rand(rows, Nn, dt=out, seed=9)
+        D = tb.grouped_gemm(0.5, A, B, _sizes(sizes), 2.0, C, transB=transB, out_dtype=out)
+        X.check(D, ref + 2.0 * C.double(), X.tolerance(ref + 2.0 * C.double(), mags, K, out, 2.0 * C))
+    assert tb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("K,Nn", [(64, 128), (200, 100), (33, 9)])
+def test_long_groups_of_few_columns(K, Nn):
+    """One CTA's long row tiles: many rows, no second block of columns."""
+    sizes = [9000, 0, 5001, 17, 6300]
+    A, B = _rand(sum(sizes) + 300, K), _rand(5, K, Nn)
+    ref, mags = X.grouped_gemm(1.0, A, B, sizes)
+    X.check(tb.grouped_gemm(1.0, A, B, _sizes(sizes)), ref, X.tolerance(ref, mags, K, BF))
+
+
 def test_whole_numbers_are_exact():
     """Small whole numbers: every partial sum is a whole number below 2^24, so
     any association gives the same result, whatever the tiling."""
@@ -170,28 +200,32 @@ def test_sizes_out_of_range_are_cut_off_and_reported():
     assert tb.device_status(0) == 0
 
 
-def test_nan_and_infinity_stay_in_their_rows_and_groups():
-    sizes, K, Nn = [50, 0, 83, 20], 192, 200
+@pytest.mark.parametrize("Nn", [200, 9000])
+def test_nan_and_infinity_stay_in_their_rows_and_groups(Nn):
+    sizes, K = [50, 0, 83, 20], 192
+    if Nn == 9000:  # CTA pairs
+        sizes = [50, 0, 383, 20]
     rows = sum(sizes) + 40
     A, B = _rand(rows, K), _rand(4, K, Nn)
     clean = tb.grouped_gemm(1.0, A, B, _sizes(sizes))
     A2, B2 = A.clone(), B.clone()
     A2[-40:] = float("nan")      # behind the last group
+    end = 50 + sizes[2]
     A2[60] = float("inf")        # one row of group 2
     B2[1] = float("nan")         # a group without rows
     B2[3] = float("inf")         # group 3
     D = tb.grouped_gemm(1.0, A2, B2, _sizes(sizes))
     keep = torch.ones(rows, dtype=torch.bool, device=DEV)
     keep[60] = False
-    keep[133:153] = False
+    keep[end:end + 20] = False
     assert torch.equal(D[keep], clean[keep])
-    assert not D[60].isfinite().any() and not D[133:153].isfinite().any()
+    assert not D[60].isfinite().any() and not D[end:end + 20].isfinite().any()
     assert (D[-40:] == 0).all()
     # the gradient of the weights: neighbours' rows are not even multiplied by zero
     dD = _rand(rows, Nn, seed=3)
     w = tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes))
     A3, d3 = A.clone(), dD.clone()
-    A3[50:133], d3[50:133] = float("inf"), float("nan")  # group 2
+    A3[50:end], d3[50:end] = float("inf"), float("nan")  # group 2
     A3[-40:], d3[-40:] = float("nan"), float("inf")
     w3 = tb.grouped_gemm_wgrad(1.0, A3, d3, _sizes(sizes))
     for g in (0, 1, 3):
@@ -351,10 +385,38 @@ def test_captured_graph_follows_the_sizes():
     assert tb.device_status(0) == 0
 
 
-def test_two_streams_and_the_same_result_twice():
+def test_captured_training_step():
+    """Forward and gradients in one captured graph, on leaves of its own."""
+    s = _sizes([30, 0, 50])
+    A, B = _rand(90, 128).requires_grad_(), _rand(3, 128, 136).requires_grad_()
+    dD = _rand(90, 136, seed=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(tb.grouped_gemm(1.0, A, B, s), (A, B), dD)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        D = tb.grouped_gemm(1.0, A, B, s)
+        dA, dB = torch.autograd.grad(D, (A, B), dD)
+    for sizes in ([30, 0, 50], [0, 90, 0], [1, 2, 3]):
+        s.copy_(torch.tensor(sizes, dtype=torch.int32))
+        with torch.no_grad():
+            A.copy_(_rand(90, 128, seed=sizes[0]))
+        graph.replay()
+        torch.cuda.synchronize()
+        a, b = A.detach(), B.detach()
+        assert torch.equal(D.detach(), tb.grouped_gemm(1.0, a, b, s))
+        assert torch.equal(dA, tb.grouped_gemm(1.0, dD, b, s, transB=True))
+        assert torch.equal(dB, tb.grouped_gemm_wgrad(1.0, a, dD, s))
+
+
+@pytest.mark.parametrize("Nn", [640, 4096])
+def test_two_streams_and_the_same_result_twice(Nn):
     sizes = [700, 0, 33, 290]
-    A, B, s = _rand(1023, 512), _rand(4, 512, 640), _sizes(sizes)
-    dD = _rand(1023, 640)
+    A, B, s = _rand(1023, 512), _rand(4, 512, Nn), _sizes(sizes)
+    dD = _rand(1023, Nn)
     want, wantw = tb.grouped_gemm(1.0, A, B, s), tb.grouped_gemm_wgrad(1.0, A, dD, s)
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
@@ -366,6 +428,32 @@ def test_two_streams_and_the_same_result_twice():
     torch.cuda.synchronize()
     for d, w in outs:
         assert torch.equal(d, want) and torch.equal(w, wantw)
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    sizes = [300, 0, 90]
+    A, B, s = _rand(390, 256), _rand(3, 256, 2304), _sizes(sizes)
+    want, wantw = tb.grouped_gemm(1.0, A, B, s), tb.grouped_gemm_wgrad(1.0, A, A, s)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                d, w = tb.grouped_gemm(1.0, A, B, s), tb.grouped_gemm_wgrad(1.0, A, A, s)
+            st.synchronize()
+        if not (torch.equal(d, want) and torch.equal(w, wantw)):
+            bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and tb.device_status(0) == 0
 
 
 def test_offsets_past_32_bits():

@@ -109,7 +109,8 @@ def test_quantise_layouts():
 
 DENSE = [(1, 128, 64), (1, 8, 32), (3, 130, 33), (17, 257, 256), (64, 128, 1000), (65, 384, 128), (200, 100, 520),
          (192, 256, 256), (385, 200, 4096), (1000, 640, 776), (448, 129, 288), (321, 300, 640),
-         (777, 4096, 520), (500, 9000, 264)]
+         (777, 4096, 520), (500, 9000, 264), (1500, 4104, 300), (400, 4100, 1000), (130, 9000, 96),
+         (9700, 128, 300), (9601, 100, 64)]
 
 
 @pytest.mark.parametrize("M,Nn,K", DENSE)
@@ -217,10 +218,29 @@ def test_grouped_gemm_mxfp4(sizes, K, Nn):
     assert tb.device_status(0) == 0
 
 
-def test_grouped_nan_stays_in_its_rows():
+@pytest.mark.parametrize("sizes", [[513, 64, 0, 255, 256, 257], [1, 0, 1290, 3], [9000, 0, 5001, 17]],
+                         ids=lambda s: f"{len(s)}x{max(s)}")
+@pytest.mark.parametrize("K,Nn", [(256, 2056), (1000, 4100), (33, 2304), (96, 128)])
+def test_grouped_gemm_mxfp4_many_tiles(sizes, K, Nn):
+    """Enough tiles for the CTA pairs (or, with few columns, one CTA's long ones)."""
+    rows = sum(sizes) + (K % 3) * 150
+    x, qb = _rand(rows, K, seed=4), _rand_mx(len(sizes), Nn, K, seed=5)
+    s = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    a = X.dequantize(*X.quantize(x), K)
+    ref, mags = X.grouped_gemm(1.0, a, _values(qb), sizes, transB=True)
+    D = tb.grouped_gemm_mxfp4(1.0, x, qb, s)
+    X.check(D, ref, X.tolerance(ref, mags, K, BF))
+    # rows quantised before: their scales are regrouped, the product is the same
+    assert torch.equal(D, tb.grouped_gemm_mxfp4(1.0, tb.quantize_mxfp4(x), qb, s))
+    assert torch.equal(D, tb.grouped_gemm_mxfp4(1.0, x, qb, s))
+    assert tb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("Nn", [136, 9000])
+def test_grouped_nan_stays_in_its_rows(Nn):
     sizes, K = [50, 0, 83, 20], 352
     s = torch.tensor(sizes, device=DEV)
-    x, qb = _rand(193, K), tb.quantize_mxfp4(_rand(4, 136, K))
+    x, qb = _rand(193, K), tb.quantize_mxfp4(_rand(4, Nn, K))
     clean = tb.grouped_gemm_mxfp4(1.0, x, qb, s)
     x2 = x.clone()
     x2[153:] = float("nan")

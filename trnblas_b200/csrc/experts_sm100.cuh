@@ -30,9 +30,9 @@
 //            tile starts at a multiple of 64 rows of its group. Each pipeline
 //            stage has its own TMEM scale columns, which its empty barrier frees
 //            with the stage. (Scale words in row order, brought and reordered
-//            by warps of the kernel, cost 1.7 times the time at 8192^3 on CTA
-//            pairs: their loads, proxy fences and arrivals were the slowest
-//            part of every stage.)
+//            by warps of the kernel, cost 2.4 times the time at 8192^3 on CTA
+//            pairs, 470 us against 197: their loads, proxy fences and arrivals
+//            were the slowest part of every stage.)
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
     // ------------------------------------------------------------ MMA issuer
     // The whole warp walks the tiles, one elected lane issues a tile's K loop:
     // one loop with warp-uniform bounds inside the election keeps descriptors
-    // and addresses in uniform registers (nested loops there did not: 130
-    // cycles an instruction on CTA pairs).
+    // and addresses in uniform registers (with both loops inside it an
+    // instruction took about 106 cycles on CTA pairs, so 17).
     const uint32_t sw0 = smem_u32(smem), sx0 = sw0 + Cfg::W_TILE;
     uint64_t wd[4], xd[4];
 #pragma unroll

@@ -295,12 +295,6 @@ int check_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64_
   return TRNBLAS_OK;
 }
 
-}  // namespace
-}  // namespace tb
-
-namespace tb {
-namespace {
-
 // Thread blocks along K: about four chunks of 256 each, so that a block has the
 // next chunk in flight behind the one it converts; one each where that leaves
 // less than two blocks an SM.
