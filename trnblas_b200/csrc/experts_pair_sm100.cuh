@@ -37,9 +37,11 @@ struct ExpPairCfg {
   static constexpr int SFX = MX ? 2 * XBLK * 512 : 0;
   static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
   static_assert(STAGE_BYTES % 1024 == 0 && BN % 32 == 0 && BN <= 256, "tile geometry");
-  // 4-bit tiles pass in half the time: two epilogue warps a TMEM lane quarter
-  static constexpr int EPI_WARPS = MX ? 8 : 4;
-  static constexpr int EPI_BYTES = EPI_WARPS * (kEpiStageBytes / 4);
+  // two a TMEM lane quarter: the last tile's epilogue runs alone, and 4-bit tiles
+  // pass in half the time (4133 rows of 8, 1024 x 2816 fp16: 23.7 us, four warps
+  // 25.4)
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int EPI_BYTES = EPI_WARPS * kExpBlockBytes;
   static constexpr int FIT = (227 * 1024 - 1024 - 512 - EPI_BYTES - kGroupTableBytes) / STAGE_BYTES;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SF_COLS = MX ? 2 * 4 * (1 + XBLK) : 0;
@@ -334,9 +336,9 @@ __global__ void __launch_bounds__(ExpPairCfg<KIND, BN, NBUF>::THREADS, 1)
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
-    // with eight warps, chunks of 32 rows alternate between two
+    // chunks of 32 rows alternate between the two
     const int c0 = 32 * ((warp - 2) >> 2), cstep = 8 * Cfg::EPI_WARPS;
-    void* tsm = epi + (warp - 2) * (kEpiStageBytes / 4);
+    void* tsm = epi + (warp - 2) * kExpBlockBytes;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     const uint32_t acce_leader = mapa_shared(smem_u32(acce_bar), 0);
     int tc = 0;

@@ -41,6 +41,7 @@ namespace tb {
 
 enum ExpKind : int { kExpF16 = 0, kExpMx4 = 1 };
 constexpr int kMaxGroups = 1024;
+constexpr int kExpBlockBytes = 2048;  // an epilogue warp's block in shared memory
 constexpr int kGroupTableBytes = (kMaxGroups + 2) * 12;
 
 struct GroupTable {
@@ -196,15 +197,16 @@ struct ExpCfg {
   static constexpr int SFX = MX ? 2 * XBLK * 512 : 0;
   static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle atom's alignment");
-  // what fits beside 16 KB of epilogue blocks and the group table; at most 8
-  static constexpr int FIT = (227 * 1024 - 1024 - 512 - kEpiStageBytes - kGroupTableBytes) / STAGE_BYTES;
+  static constexpr int EPI_BYTES = 4 * kExpBlockBytes;
+  // what fits beside the epilogue's blocks and the group table; at most 8
+  static constexpr int FIT = (227 * 1024 - 1024 - 512 - EPI_BYTES - kGroupTableBytes) / STAGE_BYTES;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SF_COLS = MX ? 2 * 4 * (1 + XBLK) : 0;  // TMEM scale columns of a stage
   static constexpr int COLS = 2 * BN + STAGES * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static_assert(COLS <= 512, "accumulators and scales fit TMEM");
   static constexpr int THREADS = 32 * 6;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + kEpiStageBytes + kGroupTableBytes;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 512 + EPI_BYTES + kGroupTableBytes;
 };
 
 // Instruction descriptor of kind::mxf4 with E8M0 scales: E2M1 operands, N / 8
@@ -252,19 +254,22 @@ __device__ __forceinline__ void exp_store(const ExpertsParams& p, int r0, int le
   if (p.out_kind == kOutF32) {
     if (wide && p.ldd % 4 == 0) {
       float* T = reinterpret_cast<float*>(tsm);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) T[j * 32 + lane] = out[j];
-      __syncwarp();
       const int q4 = (lane & 7) * 4;
       float* D = reinterpret_cast<float*>(p.D) + n0 + q4;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int row = 4 * k + (lane >> 3);
-        if (row < left)
-          *reinterpret_cast<float4*>(D + (r0 + static_cast<long long>(row)) * p.ldd) =
-              *reinterpret_cast<const float4*>(&T[row * 32 + q4]);
+      for (int h = 0; h < 32; h += 16) {  // 16 rows fill the block
+#pragma unroll
+        for (int j = 0; j < 16; ++j) T[j * 32 + lane] = out[h + j];
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 4 * k + (lane >> 3);
+          if (h + row < left)
+            *reinterpret_cast<float4*>(D + (r0 + static_cast<long long>(h + row)) * p.ldd) =
+                *reinterpret_cast<const float4*>(&T[row * 32 + q4]);
+        }
+        __syncwarp();  // the block is rewritten
       }
-      __syncwarp();  // the block is rewritten by the next chunk
       return;
     }
   } else if (wide && p.ldd % 8 == 0) {
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* epi = smem + STAGES * SB + 512;
   GroupTable tb;
-  tb.row0 = reinterpret_cast<int*>(epi + kEpiStageBytes);
+  tb.row0 = reinterpret_cast<int*>(epi + Cfg::EPI_BYTES);
   tb.tile0 = tb.row0 + kMaxGroups + 2;
   tb.blk0 = Cfg::MX ? tb.tile0 + kMaxGroups + 2 : nullptr;
 
@@ -528,7 +533,7 @@ __global__ void __launch_bounds__(ExpCfg<KIND, BN>::THREADS, 1)
   } else if (warp >= 2 && warp < 6) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;  // TMEM lane quarter
-    void* tsm = epi + (warp - 2) * (kEpiStageBytes / 4);
+    void* tsm = epi + (warp - 2) * (kExpBlockBytes);
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     int tc = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
