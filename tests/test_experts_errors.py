@@ -115,6 +115,7 @@ def test_c_entry_points_check_their_arguments():
                  (N.F32, 4, 8, FAKE, 8, FAKE + 8, 16, FAKE), (N.F32, 4, 8, FAKE, 8, FAKE, 16, FAKE + 2)):
         assert q(args[0], 1, *args[1:], None) == N.ERR_ARG, args
     assert q(N.F32, -1, 4, 8, FAKE, 8, FAKE, 16, FAKE, None) == N.ERR_ARG
+    assert q(N.F32, 1, 1, (1 << 30) + 1, FAKE, 1 << 31, FAKE, 1 << 30, FAKE, None) == N.ERR_ARG
     dq = L.trnblas_mxfp4_dequantize
     for args in ((N.F64, 4, 8, FAKE, 16, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, FAKE, FAKE, 7),
                  (N.F32, 4, 8, FAKE, 15, FAKE, FAKE, 8), (N.F32, 4, 8, FAKE, 16, None, FAKE, 8)):

@@ -176,6 +176,20 @@ def test_operands_off_16_bytes(off, step):
     X.check(db, ref, X.tolerance(ref, mags, max(sizes), BF))
 
 
+def test_single_rows_and_columns_of_any_stride():
+    flat, B = _rand(1 << 20), _rand(2, 72, 40)
+    for a in (flat.as_strided((1, 72), (1, 1)), flat.as_strided((1, 72), (1 << 19, 1)), flat.as_strided((1, 72), (9, 3)),
+              flat.as_strided((7, 72), (0, 1)), flat.as_strided((7, 72), (1, 7))):
+        sizes = [0, a.shape[0]]
+        ref, mags = X.grouped_gemm(1.0, a, B, sizes)
+        X.check(tb.grouped_gemm(1.0, a, B, _sizes(sizes)), ref, X.tolerance(ref, mags, 72, BF))
+        ref, mags = X.wgrad(1.0, a, a, sizes)
+        X.check(tb.grouped_gemm_wgrad(1.0, a, a, _sizes(sizes)), ref, X.tolerance(ref, mags, 7, BF))
+    col = flat.as_strided((9, 1), (5, 77))
+    ref, mags = X.grouped_gemm(1.0, col, _rand(1, 1, 24), [9])
+    X.check(tb.grouped_gemm(1.0, col, _rand(1, 1, 24), _sizes([9])), ref, X.tolerance(ref, mags, 1, BF))
+
+
 def test_sizes_on_host_64_bit_and_strided():
     sizes = [5, 0, 90]
     A, B = _rand(95, 64), _rand(3, 64, 64)

@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(256)
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_mx(const char* what, int64_t rows, int64_t K, int64_t ldq) {
-  const int64_t lim = (1ll << 31) - 512;
-  if (rows < 0 || K < 0 || rows > lim || K > lim) {
-    set_error(std::string(what) + ": sizes must be in [0, 2^31 - 512]");
+  // (a thread's place along K stays an int one stride past the end)
+  if (rows < 0 || K < 0 || rows > (1ll << 31) - 512 || K > (1ll << 30)) {
+    set_error(std::string(what) + ": rows must be in [0, 2^31 - 512], K in [0, 2^30]");
     return TRNBLAS_ERR_ARG;
   }
   if (ldq < round_up(K, 32) / 2 || ldq % 16) {

@@ -79,11 +79,10 @@ def _rows_operand(x: torch.Tensor):
     """(tensor, ld) of a rows x cols operand stored row by row."""
     s0, s1 = x.stride()
     rows, cols = x.shape
+    if rows == 1 and (s1 == 1 or cols == 1):
+        return x, cols  # the stride of a single row says nothing
     if s1 != 1 or s0 < cols:
-        x = x.contiguous()
-        if rows <= 1 or cols <= 1:  # strides of a single row or column say nothing
-            return x, cols
-        s0 = cols
+        return x.contiguous(), cols
     return x, s0
 
 
