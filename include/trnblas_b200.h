@@ -298,7 +298,8 @@ TRNBLAS_API int trnblas_grouped_gemm_wgrad(int dtype, int out_dtype, int64_t row
  * matrices of rows x K (X, row stride ldx in elements, F32, BF16 or F16):
  * `data` holds two values a byte, the even one in the low half, all rows ldq
  * bytes apart (a multiple of 16, at least round_up(K, 32) / 2; K is padded
- * with zeros). `scales` holds 512 bytes for every 128 rows of a matrix and
+ * with zeros up to there, and what a longer stride leaves between the rows is
+ * not touched). `scales` holds 512 bytes for every 128 rows of a matrix and
  * every 128 values of K, [matrix][row / 128][k / 128]: the four bytes of row r
  * at 16 * (r % 32) + 4 * (r / 32 % 4), zero past the rows and past K. Both on
  * 16 bytes.

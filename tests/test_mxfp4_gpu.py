@@ -304,3 +304,36 @@ def test_offsets_past_32_bits():
     a, b = X.dequantize(*X.quantize(x[-50:]), K), _values(w)
     ref = a @ b.T
     X.check(D[-50:], ref, X.tolerance(ref, a.abs() @ b.abs().T, K, BF))
+
+
+@pytest.mark.parametrize("K,ldq", [(64, 64), (33, 128), (8, 32), (300, 320), (256, 256), (1000, 512), (64, 32)])
+def test_row_strides_longer_than_the_rows(K, ldq):
+    """Through the C ABI: a stack whose packed rows lie further apart than they
+    are long. What lies between them, behind the last one and in a neighbour's
+    columns keeps its bytes; the inverse and the product read the same rows."""
+    from trnblas_b200 import _native as N
+
+    mats, rows, w = 2, 131, -(-K // 32) * 16
+    x = _rand(mats, rows, K, dt=BF)
+    want = tb.quantize_mxfp4(x)
+    buf = torch.full((mats * rows * ldq + 512,), 0xA5, dtype=torch.uint8, device=DEV)
+    scales = torch.empty_like(want.scales)
+    st = torch.cuda.current_stream().cuda_stream
+    rc = N.lib().trnblas_mxfp4_quantize(N.BF16, mats, rows, K, x.data_ptr(), K, buf.data_ptr(), ldq, scales.data_ptr(), st)
+    assert rc == 0 and torch.equal(scales, want.scales)
+    got = buf[: mats * rows * ldq].view(mats, rows, ldq)
+    assert torch.equal(got[..., :w], want.data)
+    assert (got[..., w:] == 0xA5).all() and (buf[mats * rows * ldq:] == 0xA5).all()
+    y = torch.full((mats, rows, K), 7.0, dtype=F32, device=DEV)
+    rc = N.lib().trnblas_mxfp4_dequantize(N.F32, mats, rows, K, buf.data_ptr(), ldq, scales.data_ptr(), y.data_ptr(), K, st)
+    assert rc == 0 and torch.equal(y, tb.dequantize_mxfp4(want))
+    # the second matrix as the weights of products of one and of many rows
+    q2 = tb.MXFP4Tensor(want.data[1].contiguous(), want.scales[1:].contiguous(), (rows, K))
+    for m in (1, 40):
+        a = x[0, :m].contiguous()
+        ws = torch.empty(max(1, N.lib().trnblas_mxfp4_gemm_x_workspace_size(m, 1, K, 0)), dtype=torch.uint8, device=DEV)
+        d = torch.empty(m, rows, dtype=BF, device=DEV)
+        rc = N.lib().trnblas_mxfp4_gemm_x(N.BF16, N.BF16, m, 1, rows, K, 1.0, a.data_ptr(), K, buf.data_ptr() + rows * ldq, ldq,
+                                          scales[1].data_ptr(), None, 0, 0.0, None, 0, d.data_ptr(), rows, ws.data_ptr(),
+                                          ws.numel(), st)
+        assert rc == 0 and torch.equal(d, tb.gemm_mxfp4(1.0, a, q2))

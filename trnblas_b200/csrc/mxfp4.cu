@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 4; ++i) {
       uint32_t s;
       const uint32_t w = quantize8<T>(cur[i], s);
-      if (ok[i] && (k >> 1) < ldq) *reinterpret_cast<uint32_t*>(data + row[i] * ldq + (k >> 1)) = w;
+      // up to K's last block: what follows in a longer row stride is not the row's
+      if (ok[i] && (k & ~31) < K) *reinterpret_cast<uint32_t*>(data + row[i] * ldq + (k >> 1)) = w;
       // the four scale bytes of 16 lanes; zero past K's last block
       if ((k & ~31) >= K || !ok[i]) s = 0;
       uint32_t b = s << (8 * ((lane >> 2) & 3));
