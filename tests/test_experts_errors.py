@@ -192,3 +192,14 @@ def test_oracle_quantiser_by_hand():
     v = X.dequantize(*X.quantize(x), 64)
     assert v[0, :9].tolist() == [4.0, 0.0, -1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0]
     assert v[0, 32:35].tolist() == [0.0, -(2.0 ** -128), 0.0]
+
+
+def test_row_stride_of_a_c_of_one_row():
+    from trnblas_b200.experts import _c_operand
+
+    for C in (torch.zeros(40, 1).mT, torch.zeros(3, 40, 1).mT, torch.zeros(40).as_strided((1, 40), (1, 1)),
+              torch.zeros(1, 40), torch.zeros(1).expand(1, 40)):
+        t, ld = _c_operand(C, 40)
+        assert ld >= 40 and t.stride(-1) == 1 and torch.equal(t, C)
+    t, ld = _c_operand(torch.zeros(7, 50)[:, 3:43], 40)
+    assert ld == 50 and t.storage_offset() == 3

@@ -494,3 +494,29 @@ def test_many_groups():
     dD = _rand(sum(sizes), 40)
     ref, mags = X.wgrad(1.0, A, dD, sizes)
     X.check(tb.grouped_gemm_wgrad(1.0, A, dD, _sizes(sizes)), ref, X.tolerance(ref, mags, 5, BF))
+
+
+def test_c_of_one_row_of_any_stride():
+    """A C of one row whose row stride says nothing (a transposed column), a
+    column of any stride, and stacks of them; in all four products."""
+    A, B = _rand(1, 64), _rand(2, 64, 40)
+    w, w3 = tb.quantize_mxfp4(_rand(40, 64)), tb.quantize_mxfp4(_rand(2, 40, 64))
+    s = _sizes([0, 1])
+    flat = _rand(4096)
+    for C in (flat[:40].view(40, 1).mT, flat.as_strided((1, 40), (3, 1)), flat.as_strided((1, 40), (1, 5))):
+        dense = C.clone(memory_format=torch.contiguous_format).reshape(40).view(1, 40)
+        assert dense.stride(0) == 40
+        assert torch.equal(tb.grouped_gemm(1.0, A, B, s, 2.0, C), tb.grouped_gemm(1.0, A, B, s, 2.0, dense))
+        assert torch.equal(tb.gemm_mxfp4(1.0, A, w, 2.0, C), tb.gemm_mxfp4(1.0, A, w, 2.0, dense))
+        assert torch.equal(tb.grouped_gemm_mxfp4(1.0, A, w3, s, 2.0, C), tb.grouped_gemm_mxfp4(1.0, A, w3, s, 2.0, dense))
+        ref, mags = X.grouped_gemm(1.0, A, B, [0, 1], 2.0, C)
+        X.check(tb.grouped_gemm(1.0, A, B, s, 2.0, C), ref, X.tolerance(ref, mags, 64, BF, 2.0 * C))
+    sizes = [5, 0, 2]
+    a, b = _rand(7, 1), _rand(7, 40)
+    for C in (flat[:120].view(3, 40, 1).mT, flat.as_strided((3, 1, 40), (50, 7, 1)), flat.as_strided((3, 1, 40), (0, 1, 2)),
+              flat.as_strided((3, 1, 40), (0, 1, 1))):
+        ref, mags = X.wgrad(1.0, a, b, sizes, 0.5, C)
+        X.check(tb.grouped_gemm_wgrad(1.0, a, b, _sizes(sizes), 0.5, C), ref, X.tolerance(ref, mags, 5, BF, 0.5 * C))
+    col = flat.as_strided((7, 1), (9, 5))
+    ref, mags = X.grouped_gemm(1.0, b, _rand(3, 40, 1), sizes, 1.0, col)
+    X.check(tb.grouped_gemm(1.0, b, _rand(3, 40, 1), _sizes(sizes), 1.0, col), ref, X.tolerance(ref, mags, 40, BF, col))

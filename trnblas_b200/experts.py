@@ -102,9 +102,10 @@ def _weights_operand(B: torch.Tensor, transB: bool):
 
 
 def _c_operand(C, cols: int):
-    """(tensor, ld) of a 2-D C whose rows are contiguous."""
-    c = C if C.stride(-1) == 1 and C.stride(-2) >= cols else C.contiguous()
-    return c, c.stride(-2)
+    """(tensor, ld) of a C (..., rows, cols) whose rows are contiguous."""
+    if C.stride(-1) == 1 and C.stride(-2) >= cols:
+        return C, C.stride(-2)
+    return C.contiguous(), cols  # (one row is contiguous whatever its stride says)
 
 
 def _grouped(alpha, a, B, transB, sizes, beta, C, out_dtype):
