@@ -66,3 +66,41 @@ def test_opcheck_and_parity_on_gpu():
     torch.library.opcheck(T.gemm_mxfp4, (a, d0, s0, 1.0, BF))
     assert torch.equal(T.gemm_mxfp4(a, d0, s0), tb.gemm_mxfp4(1.0, a, tb.quantize_mxfp4(w[0])))
     assert tb.device_status(0) == 0
+
+
+def test_fake_products_check_the_inner_dimension():
+    with FakeTensorMode():
+        s = torch.empty(3, device="cuda", dtype=torch.int32)
+        data, scales = T.quantize_mxfp4(torch.empty(3, 200, 100, device="cuda"))
+        d2, s2 = T.quantize_mxfp4(torch.empty(200, 100, device="cuda"))
+        x = torch.empty(7, 100, device="cuda", dtype=BF)
+        assert T.gemm_mxfp4(x, d2, s2, 1.0, BF, 100).shape == T.grouped_gemm_mxfp4(x, data, scales, s, k=100).shape == (7, 200)
+        for k, width in ((99, 100), (100, 99), (None, 96), (None, 129)):
+            y = torch.empty(7, width, device="cuda", dtype=BF)
+            for call in (lambda: T.gemm_mxfp4(y, d2, s2, k=k), lambda: T.grouped_gemm_mxfp4(y, data, scales, s, k=k)):
+                with pytest.raises(RuntimeError, match="inner dimensions"):
+                    call()
+
+
+@pytest.mark.gpu
+def test_products_check_the_weights_k():
+    """Rows of 40 values against weights of K = 64 (or the other way round) are
+    refused as the public functions refuse them; k names a K inside a block."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    s = torch.tensor([3, 4], device="cuda")
+    for K in (64, 40):
+        w = torch.randn(2, 72, K, device="cuda", generator=g)
+        q = tb.quantize_mxfp4(w)
+        q0 = tb.quantize_mxfp4(w[0])
+        x = torch.randn(7, K, device="cuda", generator=g).to(BF)
+        k = None if K == 64 else K
+        torch.library.opcheck(T.gemm_mxfp4, (x, q0.data, q0.scales, 1.0, BF, K))
+        assert torch.equal(T.gemm_mxfp4(x, q0.data, q0.scales, k=k), tb.gemm_mxfp4(1.0, x, q0))
+        assert torch.equal(T.grouped_gemm_mxfp4(x, q.data, q.scales, s, k=k), tb.grouped_gemm_mxfp4(1.0, x, q, s))
+        for y, kk in ((torch.zeros(7, 104 - K, device="cuda", dtype=BF), K), (torch.zeros(7, 40, device="cuda", dtype=BF), None),
+                      (x, 33), (x, 65)):
+            with pytest.raises(ValueError):
+                T.gemm_mxfp4(y, q0.data, q0.scales, k=kk)
+            with pytest.raises(ValueError):
+                T.grouped_gemm_mxfp4(y, q.data, q.scales, s, k=kk)
+    assert tb.device_status(0) == 0

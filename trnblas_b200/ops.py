@@ -20,7 +20,8 @@ outputs are fresh.
     grouped_gemm(a, b, group_sizes, alpha, tb, out_dtype)       rows by expert (with autograd)
     grouped_gemm_wgrad(a, b, group_sizes, alpha, out_dtype)     its weights' gradient
     quantize_mxfp4(x) -> (data, scales)           and dequantize_mxfp4(data, scales, k, dtype)
-    gemm_mxfp4(x, b_data, b_scales, alpha, out_dtype)           and grouped_gemm_mxfp4 (+ group_sizes)
+    gemm_mxfp4(x, b_data, b_scales, alpha, out_dtype, k)        and grouped_gemm_mxfp4 (+ group_sizes);
+                                                  k (the weights' K) where it is no multiple of 32
 
 `OPS[name](*args)` calls the op after the reference's operand dtype check:
 a tensor of a dtype the kernel does not take raises TypeError naming the op.
@@ -218,8 +219,9 @@ __all__ = ["OPS", "KERNEL_DTYPES", "check_kernel_operands", "gemm", "batched_gem
 
 # ── products grouped by expert and in 4 bits ────────────────────────────────
 # No counterparts in the reference, so they stand in a table of their own.
-# The 4-bit operands are the (data, scales) pairs of `MXFP4Tensor`; `rows` and
-# `k` are its logical sizes.
+# The 4-bit operands are the (data, scales) pairs of `MXFP4Tensor`, which do not
+# hold the logical K: `k` is that, checked against the other operand. Without
+# it a product's weights are as wide as their data, whole blocks of 32.
 
 
 @torch.library.custom_op("trnblas::grouped_gemm", mutates_args=(), device_types="cuda")
@@ -289,27 +291,36 @@ def _(data, scales, k, dtype):
     return data.new_empty((*data.shape[:-1], k), dtype=dtype)
 
 
+def _weights4(data, scales, k):
+    return _mx.MXFP4Tensor(data, scales, (*data.shape[:-1], 2 * data.shape[-1] if k is None else k))
+
+
+def _check_k(name, x, data, k):
+    torch._check((x.shape[1] + 31) // 32 * 16 == data.shape[-1] and k in (None, x.shape[1]),
+                 lambda: f"trnblas::{name}: inner dimensions differ")
+
+
 @torch.library.custom_op("trnblas::gemm_mxfp4", mutates_args=(), device_types="cuda")
 def gemm_mxfp4(x: torch.Tensor, b_data: torch.Tensor, b_scales: torch.Tensor, alpha: float = 1.0,
-               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    b = _mx.MXFP4Tensor(b_data, b_scales, (b_data.shape[0], x.shape[1]))
-    return _mx.gemm_mxfp4(alpha, x, b, out_dtype=out_dtype)
+               out_dtype: torch.dtype = torch.bfloat16, k: int | None = None) -> torch.Tensor:
+    return _mx.gemm_mxfp4(alpha, x, _weights4(b_data, b_scales, k), out_dtype=out_dtype)
 
 
 @gemm_mxfp4.register_fake
-def _(x, b_data, b_scales, alpha=1.0, out_dtype=torch.bfloat16):
+def _(x, b_data, b_scales, alpha=1.0, out_dtype=torch.bfloat16, k=None):
+    _check_k("gemm_mxfp4", x, b_data, k)
     return x.new_empty((x.shape[0], b_data.shape[0]), dtype=out_dtype)
 
 
 @torch.library.custom_op("trnblas::grouped_gemm_mxfp4", mutates_args=(), device_types="cuda")
 def grouped_gemm_mxfp4(x: torch.Tensor, b_data: torch.Tensor, b_scales: torch.Tensor, group_sizes: torch.Tensor,
-                       alpha: float = 1.0, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    b = _mx.MXFP4Tensor(b_data, b_scales, (b_data.shape[0], b_data.shape[1], x.shape[1]))
-    return _mx.grouped_gemm_mxfp4(alpha, x, b, group_sizes, out_dtype=out_dtype)
+                       alpha: float = 1.0, out_dtype: torch.dtype = torch.bfloat16, k: int | None = None) -> torch.Tensor:
+    return _mx.grouped_gemm_mxfp4(alpha, x, _weights4(b_data, b_scales, k), group_sizes, out_dtype=out_dtype)
 
 
 @grouped_gemm_mxfp4.register_fake
-def _(x, b_data, b_scales, group_sizes, alpha=1.0, out_dtype=torch.bfloat16):
+def _(x, b_data, b_scales, group_sizes, alpha=1.0, out_dtype=torch.bfloat16, k=None):
+    _check_k("grouped_gemm_mxfp4", x, b_data, k)
     return x.new_empty((x.shape[0], b_data.shape[1]), dtype=out_dtype)
 
 
