@@ -203,3 +203,19 @@ def test_row_stride_of_a_c_of_one_row():
         assert ld >= 40 and t.stride(-1) == 1 and torch.equal(t, C)
     t, ld = _c_operand(torch.zeros(7, 50)[:, 3:43], 40)
     assert ld == 50 and t.storage_offset() == 3
+
+
+@pytest.mark.parametrize("dual", ["A", "B", "C"])
+def test_forward_mode_is_refused(dual):
+    """A tangent is never dropped: refused before any device work, with or
+    without reverse-mode gradients and under no_grad."""
+    import torch.autograd.forward_ad as fwd
+
+    ops = {"A": A, "B": B, "C": torch.zeros(6, 4, dtype=BF)}
+    with fwd.dual_level():
+        for grad in (False, True):
+            t = ops[dual].clone().requires_grad_(grad)
+            args = {**ops, dual: fwd.make_dual(t, torch.ones_like(t))}
+            for ctx in (torch.enable_grad(), torch.no_grad()):
+                with ctx, pytest.raises(NotImplementedError, match="forward-mode"):
+                    tb.grouped_gemm(1.0, args["A"], args["B"], S, 1.0, args["C"])

@@ -520,3 +520,23 @@ def test_c_of_one_row_of_any_stride():
     col = flat.as_strided((7, 1), (9, 5))
     ref, mags = X.grouped_gemm(1.0, b, _rand(3, 40, 1), sizes, 1.0, col)
     X.check(tb.grouped_gemm(1.0, b, _rand(3, 40, 1), _sizes(sizes), 1.0, col), ref, X.tolerance(ref, mags, 40, BF, col))
+
+
+def test_forward_mode_is_refused():
+    """On the device, through the public function and the torch op; a level
+    without dual operands changes nothing."""
+    import torch.autograd.forward_ad as fwd
+
+    A, B, s = _rand(6, 64), _rand(2, 64, 32), _sizes([3, 3])
+    want = tb.grouped_gemm(1.0, A, B, s)
+    with fwd.dual_level():
+        assert torch.equal(tb.grouped_gemm(1.0, A, B, s), want)
+        for a, b in ((fwd.make_dual(A, A), B), (A, fwd.make_dual(B, B))):
+            for call in (lambda: tb.grouped_gemm(1.0, a, b, s), lambda: torch.ops.trnblas.grouped_gemm(a, b, s)):
+                with pytest.raises(NotImplementedError):
+                    call()
+        # forward over reverse: the incoming gradient carries the tangent
+        a = A.clone().requires_grad_()
+        D = tb.grouped_gemm(1.0, a, B, s)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(D, a, fwd.make_dual(torch.ones_like(want), want))

@@ -12,6 +12,7 @@ the sm_100a kernels through the C ABI; other dtypes raise TypeError.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from ._flags import trans_flag
@@ -45,6 +46,13 @@ def _same_cuda_device(*ts) -> bool:
         if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != d):
             return False
     return True
+
+
+def _refuse_tangents(name: str, *ts) -> None:
+    """The kernels see values alone: a dual tensor's tangent would be dropped."""
+    for t in ts:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
 
 
 def _check_types(name: str, a, b, out_dtype):
@@ -185,6 +193,8 @@ class _GroupedGemm(torch.autograd.Function):
         a, B, sizes = ctx.saved_tensors
         alpha, transB, beta, _ = ctx.args
         _, need_a, need_B, _, need_C = ctx.needs_input_grad
+        if forward_ad._current_level >= 0:
+            _refuse_tangents("gradient of grouped_gemm", dD)
         y = dD if dD.dtype == a.dtype else dD.to(a.dtype)
         da = dB = dC = None
         if need_a:
@@ -220,7 +230,8 @@ def grouped_gemm(
     dtype or float32 (out_dtype). alpha, beta and a same-shape C of the result's
     dtype are fused; another C is added afterwards with torch semantics.
 
-    Differentiable in A, B and C (once): the gradients run on the same kernels,
+    Differentiable in A, B and C (once, in reverse mode; tensors with forward-mode
+    tangents raise NotImplementedError): the gradients run on the same kernels,
     rounded once to their operand's dtype; an incoming float32 gradient is
     rounded to the operands' dtype first. Inside a CUDA graph capture, call
     `grouped_gemm` (transB flipped) and `grouped_gemm_wgrad` for them directly,
@@ -235,6 +246,8 @@ def grouped_gemm(
     if A.shape[1] != B.shape[2 if transB else 1]:
         raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, B {tuple(B.shape)}, transB={transB}")
     check_group_sizes(name, group_sizes, B.shape[0], A.shape[0])
+    if forward_ad._current_level >= 0:  # inside a dual level
+        _refuse_tangents(name, A, B, C)
     grad = (A.requires_grad or B.requires_grad) and torch.is_grad_enabled()
     if C is None and _same_cuda_device(A, B, group_sizes):
         if grad:
