@@ -540,3 +540,44 @@ def test_forward_mode_is_refused():
         D = tb.grouped_gemm(1.0, a, B, s)
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(D, a, fwd.make_dual(torch.ones_like(want), want))
+
+
+def test_pinned_host_operands_may_be_rewritten_after_the_call():
+    """Sizes, weights, C in pinned host memory beside rows on the device: the
+    call has read them when it returns, whatever the stream is still busy with."""
+    A, s = _rand(90, 64), [40, 0, 50]
+    B, C, C3 = _rand(3, 64, 136), _rand(90, 136, seed=2), _rand(3, 64, 136, seed=3)
+    dD, w3 = _rand(90, 136, seed=4), tb.quantize_mxfp4(_rand(3, 72, 64))
+    Cm = _rand(90, 72, seed=5)
+    for sizes, b, c, c3, cm in ((torch.tensor(s), B, C, C3, Cm), (_sizes(s), B.cpu(), C.cpu(), C3.cpu(), Cm.cpu())):
+        host = [t.pin_memory() if t.device.type == "cpu" else t for t in (sizes, b, c, c3, cm)]
+        calls = (lambda z, b, c, c3, cm: tb.grouped_gemm(1.0, A, b, z, 2.0, c),
+                 lambda z, b, c, c3, cm: tb.grouped_gemm_wgrad(1.0, A, dD, z, 2.0, c3),
+                 lambda z, b, c, c3, cm: tb.grouped_gemm_mxfp4(1.0, A, w3, z, 2.0, cm),
+                 lambda z, b, c, c3, cm: tb.grouped_gemm(1.0, A.clone().requires_grad_(), b, z, 2.0, c).detach())
+        want = [f(*(t.to(DEV) for t in host)) for f in calls]
+        for f, ref in zip(calls, want):
+            now = [t.clone().pin_memory() if t.device.type == "cpu" else t for t in host]
+            torch.cuda.synchronize()
+            torch.cuda._sleep(200_000_000)  # about 0.1 s in front of the call's copies
+            got = f(*now)
+            for t in now:
+                if t.device.type == "cpu":
+                    t.zero_()
+            torch.cuda.synchronize()
+            assert torch.equal(got, ref)
+
+
+def test_captured_graph_reads_pinned_sizes_at_each_replay():
+    A, B = _rand(90, 64), _rand(3, 64, 136)
+    s = torch.tensor([40, 0, 50]).pin_memory()
+    tb.grouped_gemm(1.0, A, B, s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        D = tb.grouped_gemm(1.0, A, B, s)
+    for z in ([40, 0, 50], [0, 90, 0], [1, 2, 3]):
+        s.copy_(torch.tensor(z))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(D, tb.grouped_gemm(1.0, A, B, _sizes(z)))

@@ -4,7 +4,7 @@
 The rows of one operand fall into groups of any length (the tokens a router
 sent to each expert), and every group has its own matrix. They stand beside
 `batched_gemm`, whose entries all have one size; the reference has no
-counterpart. The sizes stay on the device: no call synchronises with the host,
+counterpart. The sizes stay on the device: no call on device operands waits for it,
 and a captured graph follows the sizes of each replay. bfloat16 and float16 on
 the sm_100a kernels through the C ABI; other dtypes raise TypeError.
 """
@@ -16,7 +16,7 @@ from torch.autograd import forward_ad
 
 from . import _native as N
 from ._flags import trans_flag
-from .level3 import _add_c, _cuda_device, _fuse_c, _home, _mixed_dtype_error, _to
+from .level3 import _add_c, _cuda_device, _fuse_c, _home, _mixed_dtype_error
 
 DTYPES = (torch.bfloat16, torch.float16)
 MAX_GROUPS = 1024
@@ -46,6 +46,19 @@ def _same_cuda_device(*ts) -> bool:
         if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != d):
             return False
     return True
+
+
+def on_device(t, dev: torch.device, home: torch.device):
+    """t on dev, for a result on `home`. A result that stays on the device comes
+    back while the stream still runs, so the copy of a pinned tensor is waited
+    for: its owner may rewrite it after the call. A captured copy cannot be: the
+    graph reads the host memory at each replay."""
+    if not isinstance(t, torch.Tensor) or t.device == dev:
+        return t
+    if t.device.type != "cpu" or not t.is_pinned():
+        return t.to(dev)
+    with torch.cuda.device(dev):
+        return t.to(dev, non_blocking=home != dev or torch.cuda.is_current_stream_capturing())
 
 
 def _refuse_tangents(name: str, *ts) -> None:
@@ -255,7 +268,7 @@ def grouped_gemm(
         return _grouped(alpha, A, B, transB, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)
-    a, b, sizes, Cd = _to(A, dev), _to(B, dev), _to(group_sizes, dev), _to(C, dev)
+    a, b, sizes, Cd = (on_device(t, dev, home) for t in (A, B, group_sizes, C))
     fuse = _fuse_c(Cd, beta, (a.shape[0], b.shape[1] if transB else b.shape[2]), out_dtype, dev)
     c_arg = Cd if fuse else None
     if grad or (torch.is_grad_enabled() and fuse and Cd.requires_grad):
@@ -295,8 +308,8 @@ def grouped_gemm_wgrad(
         return _wgrad(alpha, A, B, group_sizes, 0.0, None, out_dtype)
     home = A.device
     dev = _cuda_device(A, B, C, group_sizes)
-    a, b, sizes, Cd = (_to(A.detach(), dev), _to(B.detach(), dev), _to(group_sizes, dev),
-                       _to(C.detach() if isinstance(C, torch.Tensor) else C, dev))
+    C = C.detach() if isinstance(C, torch.Tensor) else C
+    a, b, sizes, Cd = (on_device(t, dev, home) for t in (A.detach(), B.detach(), group_sizes, C))
     fuse = _fuse_c(Cd, beta, (sizes.shape[0], a.shape[1], b.shape[1]), out_dtype, dev)
     r = _wgrad(alpha, a, b, sizes, beta, Cd if fuse else None, out_dtype)
     if not fuse:

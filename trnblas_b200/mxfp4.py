@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _native as N
-from .experts import _c_operand, _same_cuda_device, call_on, check_group_sizes, empty
+from .experts import _c_operand, _same_cuda_device, call_on, check_group_sizes, empty, on_device
 from .level3 import _add_c, _cuda_device, _fuse_c, _home, _to
 
 BLOCK = 32
@@ -217,7 +217,7 @@ def _product(name, alpha, A, B, sizes, beta, C, out_dtype):
             B = B.to(dev)
         if A.device != dev:
             A = A.to(dev)
-        sizes, C = _to(sizes, dev), _to(C, dev)
+        sizes, C = on_device(sizes, dev, home), on_device(C, dev, home)
     rows, K = A.shape
     Nn = B.shape[-2]
     G = B.shape[0] if sizes is not None else 1
