@@ -219,3 +219,11 @@ def test_forward_mode_is_refused(dual):
             for ctx in (torch.enable_grad(), torch.no_grad()):
                 with ctx, pytest.raises(NotImplementedError, match="forward-mode"):
                     tb.grouped_gemm(1.0, args["A"], args["B"], S, 1.0, args["C"])
+
+
+@pytest.mark.parametrize("sizes", [[2 ** 62, 2 ** 62], [2 ** 63 - 1, 2 ** 63 - 1], [7, 0], [6, 1]])
+def test_host_sizes_whose_sum_wraps_around(sizes):
+    for call in (lambda s: tb.grouped_gemm(1.0, A, B, s), lambda s: tb.grouped_gemm_wgrad(1.0, A, A, s),
+                 lambda s: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), s)):
+        with pytest.raises(ValueError, match="group sizes"):
+            call(torch.tensor(sizes))

@@ -92,7 +92,8 @@ def check_group_sizes(name: str, sizes, groups: int | None, rows: int) -> None:
     if sizes.shape[0] > MAX_GROUPS:
         raise ValueError(f"{name}: at most {MAX_GROUPS} groups, got {sizes.shape[0]}")
     if sizes.device.type == "cpu" and sizes.numel():
-        if int(sizes.min()) < 0 or int(sizes.sum()) > rows:
+        # (each size first: a sum of huge ones wraps around)
+        if int(sizes.min()) < 0 or int(sizes.max()) > rows or int(sizes.sum()) > rows:
             raise ValueError(f"{name}: group sizes must not be negative nor sum to more than the {rows} rows")
 
 
