@@ -581,3 +581,36 @@ def test_captured_graph_reads_pinned_sizes_at_each_replay():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(D, tb.grouped_gemm(1.0, A, B, _sizes(z)))
+
+
+def test_unfused_c_with_and_without_gradients():
+    """A C that broadcasts or has another type is added to the rounded product;
+    whether gradients are recorded changes no value."""
+    sizes, Nn = [40, 0, 50], 136
+    A, B, s = _rand(95, 64), _rand(3, 64, Nn), _sizes(sizes)
+    dD = _rand(95, Nn, seed=1)
+    P = tb.grouped_gemm(0.7, A, B, s)
+    for C in (_rand(Nn, seed=2), _rand(95, 1, seed=3), _rand(95, Nn, dt=F32, seed=4), _rand(1, Nn, dt=F32, seed=5)):
+        want = tb.grouped_gemm(0.7, A, B, s, 0.3, C)
+        # one rounding behind the product's (a sum with an fp32 C rounds twice in fp32)
+        ref = P.double() + 0.3 * C.double()
+        tol = torch.finfo(want.dtype).eps / 2 * (ref.abs() + 0.3 * C.double().abs()) + 2.0 ** -22 * (P.double().abs() + C.double().abs())
+        assert want.dtype == torch.promote_types(BF, C.dtype) and ((want.double() - ref).abs() <= tol).all()
+        for need in ((True, False, False), (False, True, True), (False, False, True)):
+            a, b, c = (t.clone().requires_grad_(n) for t, n in zip((A, B, C), need))
+            D = tb.grouped_gemm(0.7, a, b, s, 0.3, c)
+            assert torch.equal(D.detach(), want), need
+            leaves = [t for t in (a, b, c) if t.requires_grad]
+            grads = dict(zip([i for i in range(3) if need[i]], torch.autograd.grad(D, leaves, dD.to(D.dtype))))
+            if 0 in grads:
+                assert torch.equal(grads[0], tb.grouped_gemm(0.7, dD, B, s, transB=True))
+            if 1 in grads:
+                assert torch.equal(grads[1], tb.grouped_gemm_wgrad(0.7, A, dD, s))
+            if 2 in grads:
+                x = 0.3 * dD.double()
+                ref2 = x.sum_to_size(C.shape)
+                mag = x.abs().sum_to_size(C.shape)
+                # beta * dD rounds to its type, the sum over up to 136 of them once more (fp32 inside)
+                eps = torch.finfo(C.dtype).eps
+                assert grads[2].shape == C.shape and grads[2].dtype == C.dtype
+                assert ((grads[2].double() - ref2).abs() <= (eps + 140 * 2.0 ** -24) * mag).all()

@@ -4,7 +4,7 @@
 The rows of one operand fall into groups of any length (the tokens a router
 sent to each expert), and every group has its own matrix. They stand beside
 `batched_gemm`, whose entries all have one size; the reference has no
-counterpart. The sizes stay on the device: no call on device operands waits for it,
+counterpart. The sizes stay on the device: no call on device operands synchronises,
 and a captured graph follows the sizes of each replay. bfloat16 and float16 on
 the sm_100a kernels through the C ABI; other dtypes raise TypeError.
 """
@@ -274,8 +274,8 @@ def grouped_gemm(
     c_arg = Cd if fuse else None
     if grad or (torch.is_grad_enabled() and fuse and Cd.requires_grad):
         r = _GroupedGemm.apply((alpha, transB, beta, out_dtype), a, b, sizes, c_arg)
-        if not fuse and C is not None and beta != 0.0:
-            r = r + beta * Cd
+        if not fuse:
+            r = _add_c(r, beta, Cd)
         return r if home == dev else r.to(home)
     r = _grouped(alpha, a, b, transB, sizes, beta, c_arg, out_dtype)
     if not fuse:
