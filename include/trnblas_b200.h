@@ -6,8 +6,8 @@
  * inputs without modifying them, writes only the output it is given, and
  * returns TRNBLAS_OK or a nonzero status with a message from
  * trnblas_last_error() (thread-local). Device-side failures (a bounded wait
- * that ran out) are recorded in a per-device status word read by
- * trnblas_device_status().
+ * that ran out; group sizes out of range) are recorded in a per-device status
+ * word read by trnblas_device_status().
  *
  * Matrix conventions are row-major, BLAS-style: for transX == 0, X is stored
  * rows x cols of op(X) with row stride ldX (elements); for transX != 0 it is

@@ -227,3 +227,13 @@ def test_host_sizes_whose_sum_wraps_around(sizes):
                  lambda s: tb.grouped_gemm_mxfp4(1.0, A, _mx(2, 3, 8), s)):
         with pytest.raises(ValueError, match="group sizes"):
             call(torch.tensor(sizes))
+
+
+@pytest.mark.parametrize("code,words", [(8, "group sizes"), (3, "bounded wait"), (0, None)])
+def test_status_message_names_the_cause(monkeypatch, code, words):
+    monkeypatch.setattr(N, "device_status", lambda device=None: code)
+    if words is None:
+        N.raise_on_device_status(0)
+    else:
+        with pytest.raises(RuntimeError, match=words):
+            N.raise_on_device_status(0)

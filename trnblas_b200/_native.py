@@ -189,8 +189,14 @@ def device_status(device: int | torch.device | None = None) -> int:
     return st.value
 
 
+BAD_GROUPS = 8  # the only code that is no bounded wait
+
+
 def raise_on_device_status(device=None) -> None:
-    """Raise RuntimeError if a kernel on `device` recorded a bounded-wait failure."""
+    """Raise RuntimeError if a kernel on `device` recorded a failure: a bounded
+    wait that ran out, or group sizes that it had to cut off."""
     st = device_status(device)
+    if st == BAD_GROUPS:
+        raise RuntimeError(f"trnblas_b200: group sizes on the device were negative or beyond the rows (status {st})")
     if st:
         raise RuntimeError(f"trnblas_b200: a kernel on the device gave up a bounded wait (status {st})")
