@@ -99,10 +99,10 @@ inline int fill_experts(ExpertsParams& p, int out_dtype, int64_t rows, int64_t g
 // Row tiles of 64 on single CTAs: where a group has at most 64 rows on average
 // (eight pipeline stages keep more weight bytes in flight, which is what bounds
 // a few rows a group), or where even these tiles make at most one wave. Pairs
-// otherwise. Measured, small against pair, 16 groups of m rows, K 2048, N 4096:
-// bf16 m = 16 45.1 / 47.2 us, 64 47.4 / 49.2, 96 63.9 / 51.0; MXFP4 m = 16 16.8 /
-// 17.2, 64 17.2 / 18.7, 96 26.1 / 20.7; dense MXFP4, N = K = 4096, 192 rows (96
-// small tiles) 8.4 / 10.3.
+// otherwise. Measured with weights from DRAM, small against pair, 16 groups of m
+// rows, K 2048, N 4096: bf16 m = 16 47.7 / 50.5 us, 64 49.4 / 52.9, 96 66.9 /
+// 54.6; MXFP4 m = 16 18.2 / 19.3, 64 22.3 / 23.2, 96 28.6 / 25.5; dense MXFP4, N =
+// K = 4096, 192 rows (96 small tiles) 8.8 / 11.2.
 inline bool small_tiles(int64_t rows, int64_t groups, int64_t N, bool grouped) {
   const int64_t bound = (ceil_div(rows, 64) + (grouped ? std::min(groups, rows) : 0)) * ceil_div(N, 128);
   return rows <= 64 * groups || bound <= num_sms();

@@ -38,8 +38,8 @@ struct ExpPairCfg {
   static constexpr int STAGE_BYTES = W_TILE + X_TILE + SFW + SFX;
   static_assert(STAGE_BYTES % 1024 == 0 && BN % 32 == 0 && BN <= 256, "tile geometry");
   // two a TMEM lane quarter: the last tile's epilogue runs alone, and 4-bit tiles
-  // pass in half the time (4133 rows of 8, 1024 x 2816 fp16: 23.7 us, four warps
-  // 25.4)
+  // pass in half the time (4133 rows of 8, 1024 x 2816 fp16, operands in L2: 23.7
+  // us, four warps 25.4)
   static constexpr int EPI_WARPS = 8;
   static constexpr int EPI_BYTES = EPI_WARPS * kExpBlockBytes;
   static constexpr int FIT = (227 * 1024 - 1024 - 512 - EPI_BYTES - kGroupTableBytes) / STAGE_BYTES;

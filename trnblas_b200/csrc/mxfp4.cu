@@ -431,7 +431,7 @@ int launch_mx_gemm(int out_dtype, int64_t rows, int64_t groups, int64_t N, int64
   // Pair tiles of 192 rows: two accumulators and the scales of five stages fill
   // TMEM. Where those need a second wave of pairs and tiles of 256 with one
   // accumulator do not, take these (dense: 777 rows x 4096 x 4010, 80 tiles of
-  // 192 against 64 of 256 on 74 pairs: 16.8 against 12.6 us).
+  // 192 against 64 of 256 on 74 pairs: 16.6 against 13.4 us).
   const int64_t wt = ceil_div(N, 256), pairs = num_sms() / 2;
   const bool one_wave = pair && !group_sizes && ceil_div(rows, 192) * wt > pairs && ceil_div(rows, 256) * wt <= pairs;
   const uint32_t xbox = small ? 64 : !pair ? 192 : one_wave ? 128 : 96;
