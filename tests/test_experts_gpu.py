@@ -614,3 +614,25 @@ def test_unfused_c_with_and_without_gradients():
                 eps = torch.finfo(C.dtype).eps
                 assert grads[2].shape == C.shape and grads[2].dtype == C.dtype
                 assert ((grads[2].double() - ref2).abs() <= (eps + 140 * 2.0 ** -24) * mag).all()
+
+
+def test_forward_mode_of_a_c_that_torch_adds():
+    """Where the kernels take no part, torch's own derivative stands: a C that
+    broadcasts, a C that beta = 0 does not read, and C's gradient alone."""
+    import torch.autograd.forward_ad as fwd
+
+    A, B, s = _rand(6, 64), _rand(2, 64, 32), _sizes([3, 3])
+    C, full = _rand(1, 32, seed=1), _rand(6, 32, seed=2)
+    want = tb.grouped_gemm(1.0, A, B, s, 2.0, C)
+    with fwd.dual_level():
+        for a in (A, A.clone().requires_grad_()):
+            D = tb.grouped_gemm(1.0, a, B, s, 2.0, fwd.make_dual(C, C))
+            v, t = fwd.unpack_dual(D)
+            assert torch.equal(v.detach(), want) and torch.equal(t.detach(), (2.0 * C).expand(6, 32))
+        D = tb.grouped_gemm(1.0, A, B, s, 0.0, fwd.make_dual(full, full))
+        assert torch.equal(D, tb.grouped_gemm(1.0, A, B, s)) and fwd.unpack_dual(D).tangent is None
+        with pytest.raises(NotImplementedError):
+            tb.grouped_gemm(1.0, A, B, s, 2.0, fwd.make_dual(full, full))
+        c = full.clone().requires_grad_()
+        (g,) = torch.autograd.grad(tb.grouped_gemm(1.0, A, B, s, 2.0, c), c, fwd.make_dual(want, full))
+        assert torch.equal(fwd.unpack_dual(g).primal, 2.0 * want) and torch.equal(fwd.unpack_dual(g).tangent, 2.0 * full)

@@ -207,7 +207,7 @@ class _GroupedGemm(torch.autograd.Function):
         a, B, sizes = ctx.saved_tensors
         alpha, transB, beta, _ = ctx.args
         _, need_a, need_B, _, need_C = ctx.needs_input_grad
-        if forward_ad._current_level >= 0:
+        if forward_ad._current_level >= 0 and (need_a or need_B):
             _refuse_tangents("gradient of grouped_gemm", dD)
         y = dD if dD.dtype == a.dtype else dD.to(a.dtype)
         da = dB = dC = None
@@ -260,8 +260,10 @@ def grouped_gemm(
     if A.shape[1] != B.shape[2 if transB else 1]:
         raise ValueError(f"{name}: inner dimensions differ: A {tuple(A.shape)}, B {tuple(B.shape)}, transB={transB}")
     check_group_sizes(name, group_sizes, B.shape[0], A.shape[0])
-    if forward_ad._current_level >= 0:  # inside a dual level
-        _refuse_tangents(name, A, B, C)
+    if forward_ad._current_level >= 0:  # inside a dual level (torch adds a C that is not fused)
+        D = (A.shape[0], B.shape[1 if transB else 2])
+        fused = isinstance(C, torch.Tensor) and _fuse_c(C, beta, D, out_dtype, C.device)
+        _refuse_tangents(name, A, B, C if fused else None)
     grad = (A.requires_grad or B.requires_grad) and torch.is_grad_enabled()
     if C is None and _same_cuda_device(A, B, group_sizes):
         if grad:
